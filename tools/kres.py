@@ -21,7 +21,7 @@ def main():
     csrc = os.path.join(here, "zookeeper_amd", "csrc")
     with tempfile.TemporaryDirectory() as td:
         cmd = ["/opt/rocm/bin/hipcc", "--offload-arch=gfx950", "-O3", "-std=c++17",
-               "-munsafe-fp-atomics", *flags, "-c", "-I" + csrc, "-I" + os.path.join(csrc, "kernels"),
+               "-munsafe-fp-atomics", "-Xclang", "-target-feature", "-Xclang", "-packed-fp32-ops", *flags, "-c", "-I" + csrc, "-I" + os.path.join(csrc, "kernels"),
                src, "-o", os.path.join(td, "o.o"), "-Rpass-analysis=kernel-resource-usage"]
         out = subprocess.run(cmd, capture_output=True, text=True).stderr
     rows, cur = [], None

@@ -108,7 +108,11 @@ def _compile_cmd(src: str, obj: str, extra: List[str]) -> List[str]:
     cmd = [hipcc(), "-O3", "-std=c++17", "-fPIC", "-fvisibility=hidden", "-Wall",
            "-Wno-unused-function", "-Wno-unused-variable", "-Wno-unused-result"]
     if src.endswith(".hip"):
-        cmd += [f"--offload-arch={ARCH}", "-munsafe-fp-atomics"]
+        # no packed fp32 arithmetic (v_pk_add / mul / fma_f32, which -O3 forms
+        # from ordinary float code): some of its forms have given wrong results
+        # now and then; the unpacked instructions round the same
+        cmd += [f"--offload-arch={ARCH}", "-munsafe-fp-atomics", "-Xclang", "-target-feature",
+                "-Xclang", "-packed-fp32-ops"]
     else:
         # host C++: the HIP runtime API headers (no device code, no offload)
         rocm = os.path.dirname(os.path.dirname(os.path.realpath(hipcc())))
