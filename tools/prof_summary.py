@@ -44,6 +44,7 @@ FAMILY_RULES = [
     ("ste_combine", "batch norm (apply / stats / backward)"),
     ("reduce_partials", "batch norm (apply / stats / backward)"),
     ("partials_colsum", "batch norm (apply / stats / backward)"),
+    ("ln_", "layer norm"),
     ("dw_", "depthwise conv"),
     ("pool", "pooling"),
     ("gap_", "classifier head (GAP + dense)"),

@@ -5,6 +5,7 @@ from zookeeper_amd.nn.layers import (
     BatchNorm,
     Flatten,
     GlobalAvgPool,
+    LayerNorm,
     MaxPool2d,
     QuantConv2d,
     QuantDense,
@@ -29,6 +30,7 @@ __all__ = [
     "Flatten",
     "get_quantizer",
     "GlobalAvgPool",
+    "LayerNorm",
     "magnitude_aware_sign",
     "MaxPool2d",
     "QuantConv2d",

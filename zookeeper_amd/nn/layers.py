@@ -373,6 +373,32 @@ class BatchNorm(nn.Module):
         return y
 
 
+class LayerNorm(nn.Module):
+    """Layer normalisation over the last dimension (Keras
+    ``LayerNormalization`` conventions: ``eps`` 1e-3, ``scale=False`` drops γ,
+    ``center=False`` drops β) for inputs of any leading shape; statistics in
+    fp32 (:func:`zookeeper_amd.ops.layer_norm`)."""
+
+    def __init__(self, num_features: int, eps: float = 1e-3, scale: bool = True,
+                 center: bool = True):
+        super().__init__()
+        self.num_features, self.eps = num_features, eps
+        self.weight = nn.Parameter(torch.ones(num_features)) if scale else None
+        self.bias = nn.Parameter(torch.zeros(num_features)) if center else None
+
+    def extra_repr(self) -> str:
+        return (f"{self.num_features}, eps={self.eps}, scale={self.weight is not None}, "
+                f"center={self.bias is not None}")
+
+    def forward(self, x: torch.Tensor) -> torch.Tensor:
+        from zookeeper_amd.ops import layer_norm
+
+        if x.dim() == 0 or x.shape[-1] != self.num_features:
+            raise ValueError(f"LayerNorm: expected shape (..., {self.num_features}), "
+                             f"got {tuple(x.shape)}")
+        return layer_norm(x, self.weight, self.bias, self.eps)
+
+
 class MaxPool2d(nn.Module):
     """Max pooling with TF ``same``/``valid`` padding semantics."""
 
