@@ -254,3 +254,11 @@ def test_replays_in_a_graph_and_on_another_stream():
         torch.cuda.synchronize()
         for a, e in zip(out, step(new)):
             assert torch.equal(a, e), k
+
+
+def test_second_derivative_is_refused():
+    from zookeeper_amd.ops import layer_norm
+
+    x = torch.randn(4, 32, device="cuda", requires_grad=True)
+    with pytest.raises(RuntimeError, match="not differentiable"):
+        torch.autograd.grad(layer_norm(x).sum(), x, create_graph=True)

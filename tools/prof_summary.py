@@ -45,6 +45,7 @@ FAMILY_RULES = [
     ("reduce_partials", "batch norm (apply / stats / backward)"),
     ("partials_colsum", "batch norm (apply / stats / backward)"),
     ("ln_", "layer norm"),
+    ("lp_", "token log probabilities"),
     ("dw_", "depthwise conv"),
     ("pool", "pooling"),
     ("gap_", "classifier head (GAP + dense)"),

@@ -39,12 +39,8 @@ struct Elem<2> {
 // 16 / 8 bytes at the element's own alignment: one global_load / store
 // (unaligned vector accesses are legal for global memory on gfx950; an odd row
 // length only costs the cache lines that a vector straddles).
-struct __attribute__((packed, aligned(1))) Bytes16 {
-  uint32_t v[4];
-};
-struct __attribute__((packed, aligned(1))) Bytes8 {
-  uint32_t v[2];
-};
+typedef uint32_t Bytes16 __attribute__((ext_vector_type(4), aligned(1)));
+typedef uint32_t Bytes8 __attribute__((ext_vector_type(2), aligned(1)));
 
 template <int DT>
 __device__ __forceinline__ void load8(const typename Elem<DT>::raw* p, float (&f)[8]) {
@@ -53,15 +49,15 @@ __device__ __forceinline__ void load8(const typename Elem<DT>::raw* p, float (&f
     const Bytes16 b = *reinterpret_cast<const Bytes16*>(p + 4);
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
-      f[i] = __uint_as_float(a.v[i]);
-      f[4 + i] = __uint_as_float(b.v[i]);
+      f[i] = __uint_as_float(a[i]);
+      f[4 + i] = __uint_as_float(b[i]);
     }
   } else {
     const Bytes16 a = *reinterpret_cast<const Bytes16*>(p);
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
-      f[2 * i] = Elem<DT>::up((uint16_t)(a.v[i] & 0xffffu));
-      f[2 * i + 1] = Elem<DT>::up((uint16_t)(a.v[i] >> 16));
+      f[2 * i] = Elem<DT>::up((uint16_t)(a[i] & 0xffffu));
+      f[2 * i + 1] = Elem<DT>::up((uint16_t)(a[i] >> 16));
     }
   }
 }
@@ -84,8 +80,8 @@ __device__ __forceinline__ void store8(typename Elem<DT>::raw* p, const float (&
     Bytes16 a, b;
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
-      a.v[i] = __float_as_uint(f[i]);
-      b.v[i] = __float_as_uint(f[4 + i]);
+      a[i] = __float_as_uint(f[i]);
+      b[i] = __float_as_uint(f[4 + i]);
     }
     *reinterpret_cast<Bytes16*>(p) = a;
     *reinterpret_cast<Bytes16*>(p + 4) = b;
@@ -93,7 +89,7 @@ __device__ __forceinline__ void store8(typename Elem<DT>::raw* p, const float (&
     Bytes16 a;
 #pragma unroll
     for (int i = 0; i < 4; ++i)
-      a.v[i] = (uint32_t)Elem<DT>::down(f[2 * i]) | ((uint32_t)Elem<DT>::down(f[2 * i + 1]) << 16);
+      a[i] = (uint32_t)Elem<DT>::down(f[2 * i]) | ((uint32_t)Elem<DT>::down(f[2 * i + 1]) << 16);
     *reinterpret_cast<Bytes16*>(p) = a;
   }
 }

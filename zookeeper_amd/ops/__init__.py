@@ -10,7 +10,9 @@ from zookeeper_amd.ops.binary import binary_block
 from zookeeper_amd.ops.elementwise import (chunk_table, fused_optimizer_step, normalize_flip,
                                            normalize_flip_pack)
 from zookeeper_amd.ops.layernorm import layer_norm
+from zookeeper_amd.ops.logprobs import TokenLogProbs, token_logprobs
 from zookeeper_amd.ops.xent import softmax_xent
 
 __all__ = ["available", "binary_block", "chunk_table", "fused_optimizer_step", "layer_norm",
-           "load_error", "native_disabled", "normalize_flip", "normalize_flip_pack", "softmax_xent"]
+           "load_error", "native_disabled", "normalize_flip", "normalize_flip_pack", "softmax_xent",
+           "token_logprobs", "TokenLogProbs"]

@@ -121,8 +121,11 @@ def lib() -> ctypes.CDLL:
 
 
 def stream_ptr(device: Optional[torch.device] = None) -> int:
-    """Raw ``hipStream_t`` of torch's current stream."""
-    return torch.cuda.current_stream(device).cuda_stream
+    """Raw ``hipStream_t`` of torch's current stream (without building a
+    ``torch.cuda.Stream``: 0.1 instead of 2-9 us of a small op's call)."""
+    index = device.index if device is not None else None
+    return torch._C._cuda_getCurrentRawStream(
+        torch.cuda.current_device() if index is None else index)
 
 
 def ptr(t: torch.Tensor) -> int:

@@ -69,3 +69,11 @@ def as_fp32(p):
 
 def ptr(t):
     return None if t is None else t.data_ptr()
+
+
+def once_only(what: str) -> None:
+    """Called in a backward: the kernels' gradients are not differentiable
+    themselves, so refuse ``create_graph=True`` (the only way that gradients are
+    recorded here) instead of returning constants."""
+    if torch.is_grad_enabled():
+        raise RuntimeError(f"{what}: the gradient is not differentiable (create_graph=True)")

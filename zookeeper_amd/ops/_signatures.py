@@ -112,6 +112,10 @@ SIGNATURES = {
     "zk_layer_norm_fwd": (I32, [P] * 6 + [I64, I32, I64, F32, I32, P]),
     "zk_layer_norm_bwd_ws_bytes": (I64, [I64, I32]),
     "zk_layer_norm_bwd": (I32, [P] * 9 + [I64, I64, I32, I64, I64, I32, I32, P]),
+    # log probabilities of given tokens
+    "zk_token_logprobs_ws_bytes": (I64, [I64, I32, I32]),
+    "zk_token_logprobs_fwd": (I32, [P] * 8 + [I64, I64, I32, I64, I32, I64, I32, P]),
+    "zk_token_logprobs_bwd": (I32, [P] * 6 + [I64, I32, I64, I64, I32, P]),
     # classifier head: (ReLU) + global average pool + fp32 dense layer
     "zk_head_fwd": (I32, [P, P, P, P, P] + [I32] * 5 + [P]),
     "zk_head_bwd": (I32, [P] * 8 + [I32] * 5 + [P]),

@@ -17,41 +17,41 @@ from __future__ import annotations
 from typing import Optional
 
 import torch
-from torch.autograd.function import once_differentiable
 
 from zookeeper_amd.ops._native import check, direct_grad, grad_ready, lib, stream_ptr
-from zookeeper_amd.ops._rows import (DTYPE_CODES, as_fp32, check_param, guard, ptr, rows_of,
-                                     use_kernels)
+from zookeeper_amd.ops._rows import (DTYPE_CODES, as_fp32, check_param, guard, once_only, ptr,
+                                     rows_of, use_kernels)
 
 
 def _forward(x, weight, bias, eps: float, stats: bool):
     x2, rows, stride = rows_of(x)
     cols = x.shape[-1]
     y = torch.empty(x.shape, dtype=x.dtype, device=x.device)
-    mean = rstd = None
-    if stats:
-        mean, rstd = torch.empty((2, rows), dtype=torch.float32, device=x.device).unbind(0)
+    # [2, rows]: mean, rstd
+    st = torch.empty((2, rows), dtype=torch.float32, device=x.device) if stats else None
+    mean = st.data_ptr() if stats else None
+    rstd = mean + 4 * rows if stats else None
     with guard(x):
         check(lib().zk_layer_norm_fwd(x2.data_ptr(), ptr(as_fp32(weight)), ptr(as_fp32(bias)),
-                                      y.data_ptr(), ptr(mean), ptr(rstd), rows, cols, stride,
+                                      y.data_ptr(), mean, rstd, rows, cols, stride,
                                       eps, DTYPE_CODES[x.dtype], stream_ptr(x.device)),
               "zk_layer_norm_fwd")
-    return y, mean, rstd
+    return y, st
 
 
 class _LayerNormFn(torch.autograd.Function):
     @staticmethod
     def forward(ctx, x, weight, bias, eps):
-        y, mean, rstd = _forward(x, weight, bias, eps, True)
-        ctx.save_for_backward(x, weight, mean, rstd)
+        y, stats = _forward(x, weight, bias, eps, True)
+        ctx.save_for_backward(x, weight, stats)
         # the parameters themselves: the flat gradient buffer hangs on them
         ctx.weight_param, ctx.bias_param = weight, bias
         return y
 
     @staticmethod
-    @once_differentiable
     def backward(ctx, dy):
-        x, weight, mean, rstd = ctx.saved_tensors
+        once_only("layer_norm")
+        x, weight, stats = ctx.saved_tensors
         need_x, need_w, need_b = ctx.needs_input_grad[:3]
         wp, bp = ctx.weight_param, ctx.bias_param
         dev, cols = x.device, x.shape[-1]
@@ -76,7 +76,8 @@ class _LayerNormFn(torch.autograd.Function):
             add = (1 if dw_direct is not None else 0) | (2 if db_direct is not None else 0)
             with guard(x):
                 check(lib().zk_layer_norm_bwd(dy2.data_ptr(), x2.data_ptr(), ptr(as_fp32(weight)),
-                                              mean.data_ptr(), rstd.data_ptr(), ptr(dx), ptr(dw),
+                                              stats.data_ptr(), stats.data_ptr() + 4 * rows,
+                                              ptr(dx), ptr(dw),
                                               ptr(db), ptr(ws), ws_bytes, rows, cols, xs, dys,
                                               DTYPE_CODES[x.dtype], add, stream_ptr(dev)),
                       "zk_layer_norm_bwd")
