@@ -1,0 +1,396 @@
+"""8-bit kept activations against their definitions in 64 bits.
+
+The form itself is exact arithmetic (powers of two, one rounding to a whole
+number), so packed and unpacked values are compared bit for bit.  Tolerances of
+the rest, with ``u = 2^-24`` and half a unit of the output type added:
+
+* Phi: the fitted tail is right to 1e-7 of itself, its eight Horner steps, the
+  reciprocal and the products round ~30 times, and the exponent's rounding moves
+  it by ``x^2 u`` of itself; ``1 - tail`` rounds once more.
+* matrix products: every product is exact, a sum of M of them in any order is off
+  by at most ``M`` roundings of its absolute sum (2^-23 each, should the matrix
+  unit truncate)."""
+
+import math
+
+import pytest
+import torch
+
+pytestmark = pytest.mark.gpu
+
+U = 2.0 ** -24
+DTYPES = [torch.float32, torch.bfloat16, torch.float16]
+
+
+@pytest.fixture(autouse=True)
+def _gpu():
+    if not torch.cuda.is_available():
+        pytest.skip("needs a GPU")
+    from zookeeper_amd import ops
+
+    assert ops.available(), ops.load_error()
+
+
+def _held(x):
+    """What the 8-bit form of x stands for, fp64, from its definition."""
+    n = x.shape[-1]
+    v = torch.nn.functional.pad(x.double(), (0, -n % 32)).unflatten(-1, (-1, 32))
+    top = v.abs().amax(-1)
+    fine = torch.isfinite(top)
+    t = torch.where(fine, top, torch.ones_like(top))
+    e = torch.where(t > 0, torch.frexp(t).exponent.double() - 1, torch.full_like(t, -120.0))
+    e = e.clamp(-120, 127)
+    e = e + ((torch.round(t * torch.exp2(6 - e)) >= 128) & (e < 127)).double()
+    step = torch.exp2(e - 6).unsqueeze(-1)
+    k = torch.round(v / step).clamp(-127, 127) * step
+    return k.masked_fill(~fine.unsqueeze(-1), float("nan")).flatten(-2)[..., :n]
+
+
+def _half(dt):
+    return torch.finfo(dt).eps / 2
+
+
+def _tiny(dt):
+    return torch.finfo(dt).tiny * torch.finfo(dt).eps / 2 + 2.0 ** -126
+
+
+SHAPES = [(1, 1), (1, 32), (3, 31), (2, 33), (7, 64), (5, 8), (33, 100), (1, 4097), (64, 1000),
+          (257, 96), (2047, 1111), (4, 3, 40), (1000, 2), (2, 70001)]
+
+
+@pytest.mark.parametrize("dt", DTYPES)
+@pytest.mark.parametrize("shape", SHAPES)
+def test_pack_and_unpack(shape, dt):
+    from zookeeper_amd.ops import pack8, unpack8
+
+    torch.manual_seed(sum(shape))
+    scale = torch.exp2(torch.randint(-20, 8, shape, device="cuda").float())
+    x = (torch.randn(shape, device="cuda") * scale).to(dt)
+    kept = pack8(x)
+    held = _held(x)
+    assert kept.shape == x.shape and kept.dtype == dt
+    assert torch.equal(unpack8(kept, torch.float32).double(), held)
+    assert torch.equal(unpack8(kept, torch.bfloat16).double(), held)  # exact in bf16
+    assert torch.equal(unpack8(kept), held.to(torch.float32).to(dt))
+    n = shape[-1]
+    top = torch.nn.functional.pad(x.double(), (0, -n % 32)).unflatten(-1, (-1, 32)).abs().amax(-1)
+    err = (held - x.double()).abs()
+    # half a step: 2^(E - 7) <= 2^-7 top as top >= 2^E; where the step was doubled, top
+    # rounds to 128 steps, so top >= 127.5 * 2^(E - 6) and half of 2^(E - 5) is top / 127.5
+    assert (err <= top.repeat_interleave(32, -1)[..., :n] / 127.5).all()
+    # the host's form is the same bytes
+    host = pack8(x.cpu())
+    assert torch.equal(host.codes, kept.codes.cpu()) and torch.equal(host.scales,
+                                                                     kept.scales.cpu())
+
+
+def test_pack_borders():
+    from zookeeper_amd.ops import pack8, unpack8
+
+    big = torch.finfo(torch.float32).max
+    rows = [[0.0] * 32, [-0.0] * 32, [1.0] + [0.0] * 31, [127.0, 63.5, 0.5, 1.5, 2.5],
+            [127.4999, 1.0], [127.5, 1.0], [1.9921875, -1.9921875], [1.9999999],
+            [big, -big, 1.0], [big * 2.0 ** -1], [1e-40, -1e-45], [2.0 ** -126, 2.0 ** -127],
+            [2.0 ** -120, 2.0 ** -126], [3.0] * 32]
+    x = torch.zeros(len(rows), 32, device="cuda")
+    for i, r in enumerate(rows):
+        x[i, :len(r)] = torch.tensor(r)
+    held = unpack8(pack8(x))
+    assert torch.equal(held.double(), _held(x))
+    assert torch.isfinite(held).all()
+    host = pack8(x.cpu())
+    assert torch.equal(host.codes, pack8(x).codes.cpu())
+    assert torch.equal(host.scales, pack8(x).scales.cpu())
+
+
+def test_nan_and_infinity_take_their_block_only():
+    from zookeeper_amd.ops import pack8, unpack8
+
+    for dt in DTYPES:
+        x = torch.randn(3, 100, device="cuda").to(dt)
+        x[0, 40], x[1, 99], x[2, 0] = float("nan"), float("inf"), float("-inf")
+        h = unpack8(pack8(x))
+        bad = torch.zeros(3, 100, dtype=torch.bool, device="cuda")
+        bad[0, 32:64], bad[1, 96:], bad[2, :32] = True, True, True
+        assert torch.equal(h.isnan(), bad)
+        assert torch.equal(pack8(x.cpu()).scales, pack8(x).scales.cpu())
+
+
+def _phi(x):
+    return torch.special.erfc(-x / math.sqrt(2)) / 2
+
+
+def _gelu_tols(x, dy, k, y, dx, dt):
+    tail = _phi(-x.abs())
+    ty = (_half(dt) * y.abs() + x.abs() * (tail * (1e-7 + (32 + x * x) * U) + 2 * U) + _tiny(dt))
+    tail = _phi(-k.abs())
+    dens = torch.exp(-k * k / 2) / math.sqrt(2 * math.pi)
+    slope = tail * (1e-7 + (32 + k * k) * U) + 4 * U + (k.abs() * dens) * (8 + k * k) * U
+    return ty, _half(dt) * dx.abs() + dy.abs() * slope + _tiny(dt)
+
+
+@pytest.mark.parametrize("dt", DTYPES)
+@pytest.mark.parametrize("shape", SHAPES)
+def test_gelu(shape, dt):
+    from zookeeper_amd.ops import gelu8
+
+    torch.manual_seed(sum(shape))
+    x = (torch.randn(shape, device="cuda") * 3).to(dt).requires_grad_(True)
+    dy = torch.randn(shape, device="cuda").to(dt)
+    y = gelu8(x)
+    dx, = torch.autograd.grad(y, x, dy)
+    assert y.dtype == dx.dtype == dt
+    xd, kd, dyd = x.detach().double(), _held(x.detach()), dy.double()
+    want_y = xd * _phi(xd)
+    want = dyd * (_phi(kd) + kd * torch.exp(-kd * kd / 2) / math.sqrt(2 * math.pi))
+    ty, tdx = _gelu_tols(xd, dyd, kd, want_y, want, dt)
+    assert ((y.detach().double() - want_y).abs() <= ty).all()
+    assert ((dx.double() - want).abs() <= tdx).all()
+    with torch.no_grad():
+        assert torch.equal(gelu8(x), y)
+
+
+def test_gelu_far_values_and_differences():
+    from zookeeper_amd.ops import gelu8
+
+    x = torch.tensor([[-40.0, -14.0, -6.0, 0.0, 6.0, 14.0, 40.0, 1e30, -1e30]], device="cuda")
+    y = gelu8(x)
+    want = x.double() * _phi(x.double())
+    xd = x.double()
+    tail = _phi(-xd.abs())
+    assert ((y.double() - want).abs() <= xd.abs() * tail * (1e-7 + (32 + xd * xd) * U)
+            + 4 * U * want.abs() + 2.0 ** -126).all()
+    assert torch.equal(gelu8(torch.tensor([float("inf")], device="cuda")),
+                       torch.tensor([float("inf")], device="cuda"))
+    assert gelu8(torch.full((3,), float("nan"), device="cuda")).isnan().all()
+    # values that the form holds exactly: the gradient is the function's own slope
+    x = (torch.randint(-60, 61, (4, 64), device="cuda").float() / 32)
+    x[:, ::32] = 127 / 64  # every block's step is 1 / 64
+    x.requires_grad_(True)
+    g, = torch.autograd.grad(gelu8(x).sum(), x)
+    h = 2.0 ** -8
+    with torch.no_grad():
+        d = (gelu8(x + h).double() - gelu8(x - h).double()) / (2 * h)
+    # outputs under 2 are off by under 40 u; a third derivative of at most 1.2
+    assert ((g.double() - d).abs() <= 40 * U / h + 1.2 * h * h / 6).all()
+
+
+def test_gelu_strides():
+    from zookeeper_amd.ops import gelu8
+
+    base = torch.randn(6, 5, 150, device="cuda").bfloat16()
+    for x in (base[..., 3:103], base.transpose(0, 1)[..., :64], base[:, ::2, :96],
+              base.permute(0, 2, 1), base[0, 0, :50].expand(4, 50)):
+        x = x.detach().requires_grad_(True)
+        y = gelu8(x)
+        g, = torch.autograd.grad(y.sum(), x)
+        c = x.detach().contiguous().requires_grad_(True)
+        yc = gelu8(c)
+        gc, = torch.autograd.grad(yc, c, torch.ones_like(c))
+        assert torch.equal(y, yc) and torch.equal(g, gc)
+
+
+GEMMS = [(1, 1, 1), (1, 130, 70), (33, 5, 300), (300, 128, 128), (257, 129, 127), (512, 256, 256),
+         (1000, 515, 1001), (5000, 64, 40), (40000, 16, 24), (700, 1, 600), (70, 600, 1),
+         (2049, 384, 640), (4096, 1024, 512), (64, 2048, 1536), (1300, 1000, 512)]
+
+
+@pytest.mark.parametrize("dt", DTYPES)
+@pytest.mark.parametrize("rows,outs,cols", GEMMS)
+def test_dense_gradients(rows, outs, cols, dt):
+    from zookeeper_amd.ops import dense8_grads, pack8
+
+    torch.manual_seed(rows + outs + cols)
+    x = torch.randn(rows, cols, device="cuda").to(dt)
+    dy = torch.randn(rows, outs, device="cuda").to(dt)
+    kept = pack8(x)
+    dw, db = dense8_grads(dy, kept)
+    assert dw.dtype == db.dtype == torch.float32
+    h, d = _held(x), dy.double()
+    tol = (rows + 16) * 2.0 ** -23
+    assert ((dw.double() - d.t() @ h).abs() <= tol * (d.abs().t() @ h.abs()) + 1e-30).all()
+    assert ((db.double() - d.sum(0)).abs() <= tol * d.abs().sum(0) + 1e-30).all()
+    # right on average too: a random walk of roundings, not a drift
+    rel = (dw.double() - d.t() @ h).norm() / (d.t() @ h).norm().clamp_min(1e-30)
+    assert rel <= 64 * U * max(1.0, math.sqrt(rows / 64))
+    again = dense8_grads(dy, kept, bias=False)
+    assert again[1] is None and torch.equal(again[0], dw)
+
+
+def test_dense_rows_with_gaps_and_special_values():
+    from zookeeper_amd.ops import dense8_grads, pack8
+
+    torch.manual_seed(0)
+    for dt in DTYPES:
+        base = torch.randn(200, 3, 70, device="cuda").to(dt)
+        x = torch.randn(200, 90, device="cuda").to(dt)
+        dy = base[:, 1, 3:68]
+        dw, db = dense8_grads(dy, pack8(x))
+        cw, cb = dense8_grads(dy.contiguous(), pack8(x))
+        assert torch.equal(dw, cw) and torch.equal(db, cb)
+        one = base[0, 0, :65].expand(200, 65)  # the gradient of a sum: no rows of its own
+        dw, db = dense8_grads(one, pack8(x))
+        cw, cb = dense8_grads(one.contiguous(), pack8(x))
+        assert torch.equal(dw, cw) and torch.equal(db, cb)
+        # a NaN in dy stays in its row of dw, one in x in its block's columns
+        dy = torch.randn(200, 65, device="cuda").to(dt)
+        dy[5, 7] = float("inf")
+        dw, db = dense8_grads(dy, pack8(x))
+        assert db[7].isinf() and db[:7].isfinite().all() and db[8:].isfinite().all()
+        bad = ~dw.isfinite()
+        assert bad[7].all() and not bad[:7].any() and not bad[8:].any()
+        dy[5, 7] = 1
+        x[9, 40] = float("nan")
+        dw, db = dense8_grads(dy, pack8(x))
+        assert dw[:, 32:64].isnan().all() and db.isfinite().all()
+        assert dw[:, :32].isfinite().all() and dw[:, 64:].isfinite().all()
+
+
+def test_fp32_gradients_keep_fp32_products():
+    from zookeeper_amd.ops import dense8_grads, pack8
+
+    # 24-bit values against one kept value each: the products are exact
+    dy = torch.zeros(40, 130, device="cuda")
+    dy[0] = torch.randn(130, device="cuda") * torch.exp2(
+        torch.randint(-60, 60, (130,), device="cuda").float())
+    x = torch.zeros(40, 33, device="cuda")
+    x[0, 0], x[0, 32] = 1.0, -0.5
+    dw, _ = dense8_grads(dy, pack8(x))
+    assert torch.equal(dw[:, 0], dy[0]) and torch.equal(dw[:, 32], dy[0] * -0.5)
+    assert (dw[:, 1:32] == 0).all()
+
+
+def test_dense_layer_and_autograd():
+    from zookeeper_amd.ops import dense8
+
+    torch.manual_seed(1)
+    for dt in DTYPES:
+        x = torch.randn(3, 50, 72, device="cuda").to(dt).requires_grad_(True)
+        w = (torch.randn(40, 72, device="cuda") / 8).requires_grad_(True)
+        b = torch.randn(40, device="cuda").requires_grad_(True)
+        dy = torch.randn(3, 50, 40, device="cuda").to(dt)
+        y = dense8(x, w, b)
+        assert torch.equal(y, torch.nn.functional.linear(x, w.to(dt), b.to(dt)))
+        dx, dw, db = torch.autograd.grad(y, [x, w, b], dy)
+        d = dy.double().reshape(-1, 40)
+        h = _held(x.detach()).reshape(-1, 72)
+        tol = 166 * 2.0 ** -23
+        assert dw.dtype == torch.float32
+        assert ((dw.double() - d.t() @ h).abs() <= tol * (d.abs().t() @ h.abs())).all()
+        assert ((db.double() - d.sum(0)).abs() <= tol * d.abs().sum(0)).all()
+        assert torch.equal(dx, torch.matmul(dy, w.to(dt)))
+        # only the bias wants a gradient: nothing is kept
+        y = dense8(x.detach(), w.detach(), b)
+        gb, = torch.autograd.grad(y, b, dy)
+        assert ((gb.double() - d.sum(0)).abs() <= tol * d.abs().sum(0)).all()
+        with pytest.raises(RuntimeError, match="not differentiable"):
+            torch.autograd.grad(dense8(x, w, b).sum(), w, create_graph=True)
+
+
+def test_accumulates_into_the_flat_gradient():
+    from zookeeper_amd import nn as znn
+    from zookeeper_amd.parallel.flat import FlatParams
+
+    torch.manual_seed(2)
+    for rows in (40, 9000):  # one split, several
+        m = znn.QuantDense(64, 48, use_bias=True, kept="int8").cuda()
+        x = torch.randn(rows, 64, device="cuda")
+        dy = torch.randn(rows, 48, device="cuda")
+        m(x).backward(dy)
+        gw, gb = m.weight.grad.clone(), m.bias.grad.clone()
+        FlatParams(m, torch.device("cuda"))
+        m.weight.grad.fill_(2.0)
+        m.bias.grad.fill_(-1.0)
+        m(x).backward(dy)
+        assert torch.equal(m.weight.grad, gw + 2.0) and torch.equal(m.bias.grad, gb - 1.0)
+
+
+def test_no_rows():
+    from zookeeper_amd.ops import dense8_grads, gelu8, pack8, unpack8
+
+    x = torch.randn(0, 40, device="cuda", requires_grad=True)
+    assert unpack8(pack8(x)).shape == (0, 40)
+    assert torch.autograd.grad(gelu8(x).sum(), x)[0].shape == (0, 40)
+    dw, db = dense8_grads(torch.randn(0, 30, device="cuda"), pack8(x))
+    assert torch.equal(dw, torch.zeros(30, 40, device="cuda"))
+    assert torch.equal(db, torch.zeros(30, device="cuda"))
+
+
+def test_replays_in_a_graph():
+    from zookeeper_amd.ops import dense8_grads, gelu8, pack8
+
+    torch.manual_seed(3)
+    dy = torch.randn(3000, 72, device="cuda").bfloat16()
+
+    def step(v):
+        v = v.detach().requires_grad_(True)
+        y = gelu8(v)
+        dx, = torch.autograd.grad(y, v, torch.ones_like(y))
+        return [y.detach(), dx, *dense8_grads(dy, pack8(y.detach()))]
+
+    static = torch.randn(3000, 90, device="cuda").bfloat16()
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        for _ in range(2):
+            step(static)
+    torch.cuda.current_stream().wait_stream(side)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        out = step(static)
+    for k in range(3):
+        new = torch.randn(3000, 90, device="cuda").bfloat16()
+        static.copy_(new)
+        graph.replay()
+        torch.cuda.synchronize()
+        for a, e in zip(out, step(new)):
+            assert torch.equal(a, e), k
+
+
+def test_the_operators_together():
+    """norm -> dense -> GELU -> dense -> log probabilities, all gradients, against
+    the same network of 64-bit operations on the kept values."""
+    from zookeeper_amd import nn as znn
+    from zookeeper_amd import ops
+
+    torch.manual_seed(4)
+    net = torch.nn.Sequential(znn.LayerNorm(64), znn.QuantDense(64, 96, use_bias=True, kept="int8"),
+                              znn.GELU(kept="int8"), znn.QuantDense(96, 50, use_bias=True, kept="int8"),
+                              ).cuda()
+    x = torch.randn(4, 33, 64, device="cuda")
+    t = torch.randint(0, 50, (4, 33), device="cuda")
+    acts = [x]
+    for m in net:
+        acts.append(m(acts[-1]))
+        acts[-1].retain_grad()
+    r = ops.token_logprobs(acts[-1], t)
+    loss = -(r.logp + 0.1 * r.entropy).mean()
+    loss.backward()
+
+    ln, d1, _, d2 = net
+    h0 = torch.nn.functional.layer_norm(x.double(), (64,), ln.weight.double(), ln.bias.double(),
+                                        1e-3)
+    h1 = torch.nn.functional.linear(h0, d1.weight.double(), d1.bias.double())
+    h2 = h1 * _phi(h1)
+    z = torch.nn.functional.linear(h2, d2.weight.double(), d2.bias.double()).detach()
+    z.requires_grad_(True)
+    lp = torch.log_softmax(z, -1)
+    ref = -(lp.gather(-1, t[..., None])[..., 0] - 0.1 * (lp.exp() * lp).sum(-1)).mean()
+    gz, = torch.autograd.grad(ref, z)
+    k2, k1, k0 = (_held(acts[i].detach()) for i in (3, 2, 1))
+    gh2 = gz @ d2.weight.double()
+    gh1 = gh2 * (_phi(k1) + k1 * torch.exp(-k1 * k1 / 2) / math.sqrt(2 * math.pi))
+    gh0 = gh1 @ d1.weight.double()
+    n = (x.double() - x.double().mean(-1, keepdim=True))
+    n = n / torch.sqrt(n.square().mean(-1, keepdim=True) + 1e-3)
+
+    def dw(g, k):
+        return g.reshape(-1, g.shape[-1]).t() @ k.reshape(-1, k.shape[-1])
+
+    pairs = [(loss, ref), (acts[-1].grad, gz), (d2.weight.grad, dw(gz, k2)),
+             (d2.bias.grad, gz.sum((0, 1))), (d1.weight.grad, dw(gh1, k0)),
+             (d1.bias.grad, gh1.sum((0, 1))), (ln.weight.grad, (gh0 * n).sum((0, 1))),
+             (ln.bias.grad, gh0.sum((0, 1)))]
+    for got, want in pairs:
+        # each value is a sum of at most 132 * 96 terms through five fp32 layers
+        assert (got.double() - want).norm() <= 2e-5 * want.norm()

@@ -45,6 +45,8 @@ FAMILY_RULES = [
     ("reduce_partials", "batch norm (apply / stats / backward)"),
     ("partials_colsum", "batch norm (apply / stats / backward)"),
     ("ln_", "layer norm"),
+    ("dense8_", "8-bit kept activations"),
+    ("act8_", "8-bit kept activations"),
     ("lp_", "token log probabilities"),
     ("dw_", "depthwise conv"),
     ("pool", "pooling"),

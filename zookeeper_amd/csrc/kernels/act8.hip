@@ -1,0 +1,543 @@
+// Activations kept in 8 bits for the backward pass, and the passes that use
+// them: pack / unpack, GELU forward and backward, weight and bias gradient of a
+// dense layer.
+//
+// Form.  A row is cut into blocks of 32 values; a block has one scale byte E and
+// a signed 8-bit code per value, value = code * 2^(E - 133) (the layout of the
+// OCP MXINT8 format).  E - 127 = floor(log2(max |x|)), one more where the largest
+// value would round to code 128 (so every value is within half a step; only E =
+// 254 clamps), never under E = 7 (step 2^-126: the smallest normal).  A block
+// that holds an infinity or a NaN has E = 255 and decodes to NaN.
+//
+// Why whole steps of a power of two and not e4m3: codes up to 127 and a sign are
+// exact in bf16, so a decoded tile feeds the bf16 matrix instructions without a
+// further rounding, and the error is 1 / 127.5 of the block's largest value at
+// most where e4m3's is 2^-4 of each value.
+//
+// All elementwise kernels are bound by memory.  A lane owns 8 values, the four
+// lanes of a quad a block: the block's maximum takes two DPP moves.
+#include "mfma_common.h"
+#include "rows.h"
+
+namespace {
+
+constexpr int kNT = 256;
+
+// max over the quad of lanes that shares a 32-value block
+__device__ __forceinline__ uint32_t quad_max(uint32_t v) {
+  const uint32_t a = __builtin_amdgcn_update_dpp(0, (int)v, 0xB1, 0xF, 0xF, true);
+  v = a > v ? a : v;
+  const uint32_t b = __builtin_amdgcn_update_dpp(0, (int)v, 0x4E, 0xF, 0xF, true);
+  return b > v ? b : v;
+}
+
+__device__ __forceinline__ float step_of(uint32_t E) {  // 2^(E - 133); E = 255: NaN
+  return E == 255u ? NAN : __uint_as_float((E < 7u ? 1u : E - 6u) << 23);
+}
+
+// The quad's block of 32: scale byte and this lane's 8 codes.
+__device__ __forceinline__ uint32_t encode8(const float (&x)[8], uint32_t (&code)[2]) {
+  uint32_t top = 0;
+#pragma unroll
+  for (int i = 0; i < 8; ++i) {
+    const uint32_t b = __float_as_uint(x[i]) & 0x7fffffffu;  // NaN > inf > numbers
+    top = b > top ? b : top;
+  }
+  top = quad_max(top);
+  uint32_t E = top >> 23;
+  if (E == 255u) {
+    code[0] = code[1] = 0u;
+    return 255u;
+  }
+  E = E < 7u ? 7u : E;
+  // 1 / step = 2^(133 - E); both this product and the codes' are exact
+  if (__builtin_rintf(__uint_as_float(top) * __uint_as_float((260u - E) << 23)) >= 128.f && E < 254u)
+    ++E;
+  const float inv = __uint_as_float((260u - E) << 23);
+  uint32_t c[8];
+#pragma unroll
+  for (int i = 0; i < 8; ++i) {
+    // adding 1.5 * 2^23 rounds to a whole number (ties to even) whose two's
+    // complement is in the low byte
+    const float v = __builtin_amdgcn_fmed3f(x[i] * inv, -127.f, 127.f) + 12582912.f;
+    c[i] = __float_as_uint(v) & 0xffu;
+  }
+  code[0] = c[0] | (c[1] << 8) | (c[2] << 16) | (c[3] << 24);
+  code[1] = c[4] | (c[5] << 8) | (c[6] << 16) | (c[7] << 24);
+  return E;
+}
+
+__device__ __forceinline__ float code_at(uint32_t w, int i) {
+  return (float)(int8_t)(uint8_t)(w >> (8 * i));
+}
+
+__device__ __forceinline__ void decode8(const uint32_t (&code)[2], uint32_t E, float (&x)[8]) {
+  const float s = step_of(E);
+#pragma unroll
+  for (int i = 0; i < 8; ++i) x[i] = code_at(code[i >> 2], i & 3) * s;
+}
+
+// Phi(-|x|) = t P(t) e^(-x^2 / 2) with t = 1 / (1 + 0.305 |x|) and P of degree 7,
+// fitted here to erfcx(|x| / sqrt 2) / 2 on [0, 14] (least squares, reweighted to
+// an even relative error: 1e-7).  The exponential is the normal density's too.
+__device__ __forceinline__ void normal_of(float x, float& cdf, float& e) {
+  const float t = __builtin_amdgcn_rcpf(__builtin_fmaf(0.305f, fabsf(x), 1.f));
+  e = __builtin_amdgcn_exp2f(x * x * -0.72134752044448170368f);
+  float p = 0.036698496726864566f;
+  p = __builtin_fmaf(p, t, -0.1529855293523711f);
+  p = __builtin_fmaf(p, t, 0.18571227887536676f);
+  p = __builtin_fmaf(p, t, -0.03797271523729383f);
+  p = __builtin_fmaf(p, t, 0.1210195686418104f);
+  p = __builtin_fmaf(p, t, 0.10342148895084405f);
+  p = __builtin_fmaf(p, t, 0.12246671928545089f);
+  p = __builtin_fmaf(p, t, 0.121639738931009f);
+  const float q = p * t * e;
+  cdf = x < 0.f ? q : 1.f - q;  // NaN: q is NaN
+}
+
+struct A8Args {
+  const void* in;     // x (pack, gelu fwd) / dy (gelu bwd), [rows][is]
+  void* out;          // y / dx / unpacked, [rows][D]
+  int8_t* codes;      // [rows][D]
+  uint8_t* scales;    // [rows][blocks]
+  long long rows, D, is, nv, total;  // nv: 8-value vectors of a row, padded to whole blocks
+};
+
+enum { kPack = 0, kUnpack = 1, kGeluFwd = 2, kGeluKeep = 3, kGeluBwd = 4 };
+
+template <int DT, int OP>
+__global__ __launch_bounds__(kNT) void act8_kernel(A8Args a) {
+  typedef typename Elem<DT>::raw raw;
+  const long long step = (long long)gridDim.x * kNT;
+  for (long long id = (long long)blockIdx.x * kNT + threadIdx.x; id < a.total; id += step) {
+    long long row = 0, v = id;
+    if (a.rows > 1) {  // uniform
+      if (a.total < (1LL << 31)) {
+        row = (uint32_t)id / (uint32_t)a.nv;
+      } else {
+        row = id / a.nv;
+      }
+      v = id - row * a.nv;
+    }
+    const long long c = v * 8;
+    const int n = (int)(a.D - c < 8 ? a.D - c : 8);  // <= 0 behind the row's end
+    const long long at = row * a.D + c;
+    const long long sc = row * (a.nv >> 2) + (v >> 2);
+    float x[8];
+    if constexpr (OP != kUnpack) {
+      load8_n<DT>(reinterpret_cast<const raw*>(a.in) + row * a.is + c, n, 0.f, x);
+    }
+    if constexpr (OP == kPack || OP == kGeluKeep) {
+      uint32_t w[2];
+      const uint32_t E = encode8(x, w);
+      if (n >= 8) {
+        Bytes8 b;
+        b[0] = w[0];
+        b[1] = w[1];
+        *reinterpret_cast<Bytes8*>(a.codes + at) = b;
+      } else {
+#pragma unroll
+        for (int i = 0; i < 8; ++i)
+          if (i < n) a.codes[at + i] = (int8_t)(uint8_t)(w[i >> 2] >> (8 * (i & 3)));
+      }
+      if ((v & 3) == 0) a.scales[sc] = (uint8_t)E;
+    }
+    if constexpr (OP == kUnpack || OP == kGeluBwd) {
+      uint32_t w[2] = {0u, 0u};
+      if (n >= 8) {
+        const Bytes8 b = *reinterpret_cast<const Bytes8*>(a.codes + at);
+        w[0] = b[0];
+        w[1] = b[1];
+      } else {
+#pragma unroll
+        for (int i = 0; i < 8; ++i)
+          if (i < n) w[i >> 2] |= (uint32_t)(uint8_t)a.codes[at + i] << (8 * (i & 3));
+      }
+      float k[8];
+      decode8(w, a.scales[sc], k);
+#pragma unroll
+      for (int i = 0; i < 8; ++i) {
+        if constexpr (OP == kUnpack) {
+          x[i] = k[i];
+        } else {
+          float cdf, e;
+          normal_of(k[i], cdf, e);
+          x[i] *= cdf + k[i] * e * 0.39894228040143267794f;
+        }
+      }
+    }
+    if constexpr (OP == kGeluFwd || OP == kGeluKeep) {
+#pragma unroll
+      for (int i = 0; i < 8; ++i) {
+        float cdf, e;
+        normal_of(x[i], cdf, e);
+        x[i] *= cdf;
+      }
+    }
+    if constexpr (OP != kPack) {
+      if (n > 0) store8_n<DT>(reinterpret_cast<raw*>(a.out) + at, n, x);
+    }
+  }
+}
+
+template <int OP>
+int act8_launch(const void* in, void* out, void* codes, void* scales, long long rows,
+                long long D, long long is, int dt, hipStream_t st) {
+  if (rows < 0 || D < 1 || is < 0 || dt < 0 || dt > 2) return (int)hipErrorInvalidValue;
+  if (rows == 0) return 0;
+  // whole blocks and no gaps: one long row (no division)
+  if (D % 32 == 0 && (is == D || rows == 1)) {
+    D *= rows;
+    is = D;
+    rows = 1;
+  }
+  A8Args a{in, out, (int8_t*)codes, (uint8_t*)scales, rows, D, is, (D + 31) / 32 * 4, 0};
+  a.total = rows * a.nv;
+  long long blocks = (a.total + kNT - 1) / kNT;
+  if (blocks > (1 << 20)) blocks = 1 << 20;
+  const dim3 g((unsigned)blocks);
+  if (dt == 0) hipLaunchKernelGGL((act8_kernel<0, OP>), g, dim3(kNT), 0, st, a);
+  if (dt == 1) hipLaunchKernelGGL((act8_kernel<1, OP>), g, dim3(kNT), 0, st, a);
+  if (dt == 2) hipLaunchKernelGGL((act8_kernel<2, OP>), g, dim3(kNT), 0, st, a);
+  return (int)hipGetLastError();
+}
+
+// ===========================================================================
+// Weight gradient of a dense layer from its kept input:
+//   dW[n][k] = sum_m dy[m][n] x8[m][k],   db[n] = sum_m dy[m][n]
+// A matrix product whose reduction runs over the rows of both operands.  A
+// block owns a 128 x 128 tile of dW and walks 32 rows a step: dy and the decoded
+// codes go through registers into LDS as [m][column] bf16 rows (256 B, swizzled
+// by tr_swz so that the transposed reads have no bank conflicts), the fragments
+// (8 consecutive m of a column) come from ds_read_b64_tr_b16.
+//
+// dy in fp16 / fp32 is cut into 2 / 3 bf16 terms by truncation (8 significant
+// bits each: 11 and 24 bits are exact), one matrix product per term into the same
+// accumulators; x8 is exact in bf16 and needs one.  So fp32 gradients keep fp32
+// products at a third of the bf16 rate.
+//
+// db comes from the same fragments times a column of ones; the k-tiles of one
+// n-tile share the rows' steps for it.
+//
+// Few tiles: the rows are split, every split writes its partial tile and a
+// second launch adds them in order (no atomics).
+// ===========================================================================
+typedef float f32x4 __attribute__((ext_vector_type(4)));
+
+constexpr int kT = 128;       // tile edge, n and k
+constexpr int kMS = 32;       // rows a step
+constexpr int kPlane = kMS * kT * 2;
+
+struct D8Args {
+  const void* dy;         // [M][dys]
+  const int8_t* codes;    // [M][K]
+  const uint8_t* scales;  // [M][kb]
+  float* dw;              // [N][K]
+  float* db;              // [N] or null
+  float* slab;            // [splits][N][K], then [splits * ktiles][N] for db
+  long long dys;
+  long long M;
+  int N, K, kb, ntiles, ktiles, splits, add;
+  long long mps;          // rows of a split (multiple of kMS)
+};
+
+__device__ __forceinline__ f32x4 mma16(const uint4& a, const uint4& b, const f32x4& c) {
+  return __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8, a),
+                                                 __builtin_bit_cast(bf16x8, b), c, 0, 0, 0);
+}
+
+// 8 consecutive m of column c0 + (lane & 15) from a swizzled [m][128] bf16 plane:
+// lane l: m = 8 (l >> 4) ..
+__device__ __forceinline__ uint4 col_frag(const unsigned char* plane, int c0, int lane) {
+  const int g = lane >> 4, i = lane & 15, q = i >> 2, p = i & 3;
+  const int r0 = 8 * g + q, r1 = r0 + 4;
+  const int slot = (c0 >> 3) | (p >> 1), inner = (p & 1) * 8;
+  const int o0 = r0 * 256 + ((slot ^ tr_swz<256>(r0)) << 4) + inner;
+  const int o1 = r1 * 256 + ((slot ^ tr_swz<256>(r1)) << 4) + inner;
+  typedef __attribute__((address_space(3))) s16x4 lds_s16x4;
+  const s16x4 lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16(
+      (lds_s16x4*)(uintptr_t)(const __attribute__((address_space(3))) void*)(plane + o0));
+  const s16x4 hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16(
+      (lds_s16x4*)(uintptr_t)(const __attribute__((address_space(3))) void*)(plane + o1));
+  const s16x8 v = {lo[0], lo[1], lo[2], lo[3], hi[0], hi[1], hi[2], hi[3]};
+  return __builtin_bit_cast(uint4, v);
+}
+
+// The first bf16 term of f (8 leading bits, never an overflow) and the exact rest;
+// an infinity or NaN has no rest.
+__device__ __forceinline__ uint32_t cut_term(float& f) {
+  const uint32_t u = __float_as_uint(f);
+  uint32_t h = u & 0xffff0000u;
+  if ((u & 0x7f800000u) == 0x7f800000u) {
+    if (u & 0x007fffffu) h |= 0x00400000u;  // NaN stays one
+    f = 0.f;
+  } else {
+    f -= __uint_as_float(h);
+  }
+  return h >> 16;
+}
+
+template <int DT>
+__global__ __launch_bounds__(kNT, 2) void dense8_wgrad_kernel(D8Args a) {
+  typedef typename Elem<DT>::raw raw;
+  constexpr int TERMS = DT == 1 ? 1 : DT == 2 ? 2 : 3;
+  constexpr int BUF = (TERMS + 1) * kPlane;
+  __shared__ __attribute__((aligned(1024))) unsigned char smem[2 * BUF];
+  const int tid = threadIdx.x, wave = tid >> 6, lane = tid & 63;
+  const int wn = wave >> 1, wk = wave & 1;
+  const int L = xcd_linear(blockIdx.x, gridDim.x);
+  const int tiles = a.ntiles * a.ktiles;
+  const int split = L / tiles, tile = L - split * tiles;
+  const int kt = tile % a.ktiles, nt = tile / a.ktiles;
+  const int n0 = nt * kT, k0 = kt * kT;
+  const long long m0 = split * a.mps, m1 = min(a.M, m0 + a.mps);
+  const int steps = (int)((m1 - m0 + kMS - 1) / kMS);
+
+  // staging: dy rows tid / 16 and + 16, columns 8 (tid % 16); codes row tid / 8,
+  // columns 16 (tid % 8)
+  const int dr = tid >> 4, dc = (tid & 15) * 8, xr = tid >> 3, xc = (tid & 7) * 16;
+  const int dn = a.N - n0 - dc, xn = a.K - k0 - xc;
+  const raw* dyp = reinterpret_cast<const raw*>(a.dy) + n0 + dc;
+  const int8_t* cp = a.codes + k0 + xc;
+  const uint8_t* sp = a.scales + ((k0 + xc) >> 5);
+  float dreg[2][8];
+  uint32_t creg[4], ereg;
+  auto load = [&](int s) {
+    const long long m = m0 + (long long)s * kMS;
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+      const long long r = m + dr + 16 * i;
+      load8_n<DT>(dyp + r * a.dys, r < m1 ? dn : 0, 0.f, dreg[i]);
+    }
+    const long long r = m + xr;
+    const int n = r < m1 ? xn : 0;
+    creg[0] = creg[1] = creg[2] = creg[3] = 0u;
+    ereg = 7u;
+    if (n > 0) {
+      const int8_t* p = cp + r * a.K;
+      ereg = sp[r * a.kb];
+      if (n >= 16) {
+        const Bytes16 b = *reinterpret_cast<const Bytes16*>(p);
+#pragma unroll
+        for (int i = 0; i < 4; ++i) creg[i] = b[i];
+      } else {
+#pragma unroll
+        for (int i = 0; i < 16; ++i)
+          if (i < n) creg[i >> 2] |= (uint32_t)(uint8_t)p[i] << (8 * (i & 3));
+      }
+    }
+  };
+  auto store = [&](int s) {
+    unsigned char* buf = smem + (s & 1) * BUF;
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+      const int r = dr + 16 * i;
+      const int o = r * 256 + (((tid & 15) ^ tr_swz<256>(r)) << 4);
+      if constexpr (TERMS == 1) {
+        uint4 w;
+        w.x = zk::pack_bf16x2(dreg[i][0], dreg[i][1]);
+        w.y = zk::pack_bf16x2(dreg[i][2], dreg[i][3]);
+        w.z = zk::pack_bf16x2(dreg[i][4], dreg[i][5]);
+        w.w = zk::pack_bf16x2(dreg[i][6], dreg[i][7]);
+        *reinterpret_cast<uint4*>(buf + o) = w;
+      } else {
+#pragma unroll
+        for (int t = 0; t < TERMS; ++t) {
+          uint32_t h[8];
+#pragma unroll
+          for (int j = 0; j < 8; ++j) h[j] = cut_term(dreg[i][j]);
+          const uint4 w = {h[0] | (h[1] << 16), h[2] | (h[3] << 16), h[4] | (h[5] << 16),
+                           h[6] | (h[7] << 16)};
+          *reinterpret_cast<uint4*>(buf + t * kPlane + o) = w;
+        }
+      }
+    }
+    const float step = step_of(ereg);
+    unsigned char* xb = buf + TERMS * kPlane;
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+      uint32_t w[4];
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        const uint32_t c = creg[2 * h + (j >> 1)];
+        w[j] = zk::pack_bf16x2(code_at(c, 2 * (j & 1)) * step, code_at(c, 2 * (j & 1) + 1) * step);
+      }
+      *reinterpret_cast<uint4*>(xb + xr * 256 +
+                                ((((tid & 7) * 2 + h) ^ tr_swz<256>(xr)) << 4)) =
+          uint4{w[0], w[1], w[2], w[3]};
+    }
+  };
+
+  f32x4 acc[4][4], bacc[4];
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    bacc[i] = f32x4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+    for (int j = 0; j < 4; ++j) acc[i][j] = f32x4{0.f, 0.f, 0.f, 0.f};
+  }
+  const uint4 ones = {0x3F803F80u, 0x3F803F80u, 0x3F803F80u, 0x3F803F80u};
+
+  if (steps > 0) load(0);
+  for (int s = 0; s < steps; ++s) {
+    store(s);
+    __syncthreads();
+    if (s + 1 < steps) load(s + 1);
+    const unsigned char* buf = smem + (s & 1) * BUF;
+    uint4 x[4];
+#pragma unroll
+    for (int j = 0; j < 4; ++j) x[j] = col_frag(buf + TERMS * kPlane, wk * 64 + j * 16, lane);
+    const bool sum = a.db && wk == 0 && s % a.ktiles == kt;
+#pragma unroll
+    for (int t = 0; t < TERMS; ++t) {
+      uint4 d[4];
+#pragma unroll
+      for (int i = 0; i < 4; ++i) d[i] = col_frag(buf + t * kPlane, wn * 64 + i * 16, lane);
+#pragma unroll
+      for (int i = 0; i < 4; ++i)
+#pragma unroll
+        for (int j = 0; j < 4; ++j) acc[i][j] = mma16(d[i], x[j], acc[i][j]);
+      if (sum)
+#pragma unroll
+        for (int i = 0; i < 4; ++i) bacc[i] = mma16(d[i], ones, bacc[i]);
+    }
+    // the next store goes to the other buffer: its readers passed the barrier above
+  }
+
+  const bool direct = a.splits == 1;
+  float* out = direct ? a.dw : a.slab + (long long)split * a.N * a.K;
+  const bool add = direct && (a.add & 1);
+#pragma unroll
+  for (int i = 0; i < 4; ++i)
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+      const int n = n0 + wn * 64 + i * 16 + 4 * (lane >> 4) + e;
+      if (n >= a.N) continue;
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        const int k = k0 + wk * 64 + j * 16 + (lane & 15);
+        if (k < a.K) {
+          float* o = out + (long long)n * a.K + k;
+          *o = add ? *o + acc[i][j][e] : acc[i][j][e];
+        }
+      }
+    }
+  if (a.db && wk == 0 && (lane & 15) == 0) {
+    float* part = a.slab + (direct ? 0 : (long long)a.splits * a.N * a.K) +
+                  ((long long)split * a.ktiles + kt) * a.N;
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        const int n = n0 + wn * 64 + i * 16 + 4 * (lane >> 4) + e;
+        if (n < a.N) part[n] = bacc[i][e];
+      }
+  }
+}
+
+// out[i] (+)= sum over p of part[p][i]: 16 slices of the parts side by side, each in
+// order, joined in order
+__global__ __launch_bounds__(1024) void dense8_sum_kernel(const float* __restrict__ part,
+                                                          int parts, long long n,
+                                                          float* __restrict__ out, int add) {
+  __shared__ float red[16][64];
+  const int col = threadIdx.x & 63, sl = threadIdx.x >> 6;
+  const long long i = (long long)blockIdx.x * 64 + col;
+  float s = 0.f;
+  if (i < n)
+    for (int p = sl; p < parts; p += 16) s += part[(long long)p * n + i];
+  red[sl][col] = s;
+  __syncthreads();
+  if (sl == 0 && i < n) {
+#pragma unroll
+    for (int o = 1; o < 16; ++o) s += red[o][col];
+    out[i] = add ? out[i] + s : s;
+  }
+}
+
+struct D8Plan {
+  int ntiles, ktiles, splits;
+  long long mps, slab, bytes;
+};
+
+// Two blocks per CU, at least 256 rows per split.
+D8Plan dense8_plan(long long M, int N, int K) {
+  D8Plan p;
+  p.ntiles = (N + kT - 1) / kT;
+  p.ktiles = (K + kT - 1) / kT;
+  const long long tiles = (long long)p.ntiles * p.ktiles;
+  long long s = (512 + tiles - 1) / tiles;
+  const long long most = (M + 255) / 256;
+  if (s > most) s = most;
+  if (s < 1) s = 1;
+  p.mps = ((M + s - 1) / s + kMS - 1) / kMS * kMS;
+  p.splits = (int)((M + p.mps - 1) / p.mps);
+  p.slab = p.splits > 1 ? (long long)p.splits * N * K : 0;
+  p.bytes = 4 * (p.slab + (long long)p.splits * p.ktiles * N);
+  return p;
+}
+
+bool dense8_ok(long long M, int N, int K) {
+  return M >= 1 && N >= 1 && K >= 1 && M < (1LL << 31) && N < (1 << 24) && K < (1 << 24) &&
+         ((N + kT - 1LL) / kT) * ((K + kT - 1LL) / kT) < (1 << 20);
+}
+
+}  // namespace
+
+// x [rows][xs] -> codes [rows][D], scales [rows][ceil(D / 32)]; dt: 0 fp32, 1
+// bf16, 2 fp16.
+ZK_EXPORT int zk_pack8(const void* x, void* codes, void* scales, long long rows, long long D,
+                       long long xs, int dt, hipStream_t st) {
+  return act8_launch<kPack>(x, nullptr, codes, scales, rows, D, xs, dt, st);
+}
+
+ZK_EXPORT int zk_unpack8(const void* codes, const void* scales, void* out, long long rows,
+                         long long D, int dt, hipStream_t st) {
+  return act8_launch<kUnpack>(nullptr, out, const_cast<void*>(codes), const_cast<void*>(scales),
+                              rows, D, D, dt, st);
+}
+
+// y = x Phi(x); codes / scales (both or neither): the 8-bit form of x.
+ZK_EXPORT int zk_gelu8_fwd(const void* x, void* y, void* codes, void* scales, long long rows,
+                           long long D, long long xs, int dt, hipStream_t st) {
+  return codes ? act8_launch<kGeluKeep>(x, y, codes, scales, rows, D, xs, dt, st)
+               : act8_launch<kGeluFwd>(x, y, nullptr, nullptr, rows, D, xs, dt, st);
+}
+
+// dx = dy (Phi(x8) + x8 phi(x8))
+ZK_EXPORT int zk_gelu8_bwd(const void* dy, const void* codes, const void* scales, void* dx,
+                           long long rows, long long D, long long dys, int dt, hipStream_t st) {
+  return act8_launch<kGeluBwd>(dy, dx, const_cast<void*>(codes), const_cast<void*>(scales), rows, D,
+                               dys, dt, st);
+}
+
+// Workspace bytes of zk_dense8_wgrad, or -1 for sizes it does not take.
+ZK_EXPORT long long zk_dense8_wgrad_ws_bytes(long long M, int N, int K) {
+  return dense8_ok(M, N, K) ? dense8_plan(M, N, K).bytes : -1;
+}
+
+// dw [N][K] and db [N] (or null), fp32, from dy [M][dys] and the kept input
+// [M][K].  add: bit 0 dw, bit 1 db are accumulated into instead of written.
+ZK_EXPORT int zk_dense8_wgrad(const void* dy, const void* codes, const void* scales, void* dw,
+                              void* db, void* ws, long long ws_bytes, long long M, int N, int K,
+                              long long dys, int dt, int add, hipStream_t st) {
+  if (!dense8_ok(M, N, K) || dys < 0 || dt < 0 || dt > 2) return (int)hipErrorInvalidValue;
+  const D8Plan p = dense8_plan(M, N, K);
+  if (!ws || ws_bytes < p.bytes) return (int)hipErrorInvalidValue;
+  D8Args a{dy, (const int8_t*)codes, (const uint8_t*)scales, (float*)dw, (float*)db, (float*)ws,
+           dys, M, N, K, (K + 31) / 32, p.ntiles, p.ktiles, p.splits, add, p.mps};
+  const dim3 g((unsigned)((long long)p.ntiles * p.ktiles * p.splits));
+  if (dt == 0) hipLaunchKernelGGL(dense8_wgrad_kernel<0>, g, dim3(kNT), 0, st, a);
+  if (dt == 1) hipLaunchKernelGGL(dense8_wgrad_kernel<1>, g, dim3(kNT), 0, st, a);
+  if (dt == 2) hipLaunchKernelGGL(dense8_wgrad_kernel<2>, g, dim3(kNT), 0, st, a);
+  ZK_CHECK_LAUNCH();
+  const long long n = (long long)N * K;
+  if (p.splits > 1)
+    hipLaunchKernelGGL(dense8_sum_kernel, dim3((unsigned)((n + 63) / 64)), dim3(1024), 0, st,
+                       (const float*)ws, p.splits, n, (float*)dw, add & 1);
+  if (db)
+    hipLaunchKernelGGL(dense8_sum_kernel, dim3((unsigned)((N + 63) / 64)), dim3(1024), 0, st,
+                       (const float*)ws + p.slab, p.splits * p.ktiles, (long long)N, (float*)db,
+                       (add >> 1) & 1);
+  ZK_CHECK_LAUNCH();
+  return 0;
+}

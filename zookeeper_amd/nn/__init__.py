@@ -4,6 +4,7 @@ from zookeeper_amd.nn.layers import (
     AvgPool2d,
     BatchNorm,
     Flatten,
+    GELU,
     GlobalAvgPool,
     LayerNorm,
     MaxPool2d,
@@ -28,6 +29,7 @@ __all__ = [
     "AvgPool2d",
     "BatchNorm",
     "Flatten",
+    "GELU",
     "get_quantizer",
     "GlobalAvgPool",
     "LayerNorm",

@@ -254,8 +254,17 @@ class QuantConv2d(nn.Module):
             CONSTRAINTS[self.kernel_constraint](self.weight)
 
 
+def _check_kept(kept: Optional[str]) -> Optional[str]:
+    if kept not in (None, "int8"):
+        raise ValueError(f"kept must be None or 'int8', got {kept!r}")
+    return kept
+
+
 class QuantDense(nn.Module):
-    """Fully-connected layer with optional quantizers (Larq ``QuantDense``)."""
+    """Fully-connected layer with optional quantizers (Larq ``QuantDense``).
+
+    ``kept="int8"`` (float layers only) keeps the input in 8 bits for the
+    weight gradient (:func:`zookeeper_amd.ops.dense8`)."""
 
     def __init__(
         self,
@@ -266,8 +275,12 @@ class QuantDense(nn.Module):
         kernel_constraint: Optional[str] = None,
         use_bias: bool = False,
         kernel_initializer: str = "glorot_normal",
+        kept: Optional[str] = None,
     ):
         super().__init__()
+        self.kept = _check_kept(kept)
+        if kept is not None and (input_quantizer is not None or kernel_quantizer is not None):
+            raise ValueError("kept='int8' is for float layers: the quantizers must be None")
         self.in_features, self.out_features = in_features, out_features
         self.input_quantizer_name = input_quantizer if isinstance(input_quantizer, str) else None
         self.kernel_quantizer_name = kernel_quantizer if isinstance(kernel_quantizer, str) else None
@@ -287,6 +300,10 @@ class QuantDense(nn.Module):
             if bconv.dense_supported(x, self.weight, self.bias):
                 clip = getattr(self, "clip_value", 1.0)
                 return bconv.binary_dense(x, self.weight, clip, clip, owner=self)
+        if self.kept is not None:
+            from zookeeper_amd.ops import dense8
+
+            return dense8(x, self.weight, self.bias)
         if self.input_quantizer is not None:
             x = self.input_quantizer(x)
         w = self.weight
@@ -397,6 +414,25 @@ class LayerNorm(nn.Module):
             raise ValueError(f"LayerNorm: expected shape (..., {self.num_features}), "
                              f"got {tuple(x.shape)}")
         return layer_norm(x, self.weight, self.bias, self.eps)
+
+
+class GELU(nn.Module):
+    """``x * Phi(x)``.  ``kept="int8"`` keeps the input in 8 bits for the backward
+    (:func:`zookeeper_amd.ops.gelu8`)."""
+
+    def __init__(self, kept: Optional[str] = None):
+        super().__init__()
+        self.kept = _check_kept(kept)
+
+    def extra_repr(self) -> str:
+        return f"kept={self.kept!r}"
+
+    def forward(self, x: torch.Tensor) -> torch.Tensor:
+        if self.kept is None:
+            return F.gelu(x)
+        from zookeeper_amd.ops import gelu8
+
+        return gelu8(x)
 
 
 class MaxPool2d(nn.Module):

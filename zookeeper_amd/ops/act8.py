@@ -1,0 +1,324 @@
+"""Activations kept in 8 bits for the backward pass (``csrc/kernels/act8.hip``).
+
+What a layer saves for its backward pass is most of a training step's memory;
+here it is one signed byte per value and one scale byte per 32 instead of 2 or 4
+bytes per value.
+
+* :func:`pack8` / :func:`unpack8` -- the form itself (:class:`Packed8`): blocks
+  of 32 values along the last dimension share a power-of-two step, every value
+  is within half a step of what it stands for, and half a step is at most 1 /
+  127.5 of the block's largest value (or 2^-127).  A block with an infinity or a NaN stands for
+  NaN.
+* :func:`gelu8` -- GELU (the exact form ``x * Phi(x)``) that keeps its input in 8
+  bits; the same pass over ``x`` writes the output and the kept form.
+* :func:`dense8` -- a dense layer that keeps its input in 8 bits; its weight
+  gradient ``dy^T x8`` and bias gradient come from :func:`dense8_grads`, a matrix
+  product that decodes the kept input on its way to the matrix units.
+
+Forward results are exact (they use the unrounded input); gradients are those
+of the kept input.  ``dense8`` computes ``y`` and ``dx`` with the library's
+matrix products, like the framework's other dense layers.  Host tensors run the
+same definitions in PyTorch.
+"""
+
+from __future__ import annotations
+
+import math
+from typing import Optional, Tuple
+
+import torch
+import torch.nn.functional as F
+
+from zookeeper_amd.ops._native import check, direct_grad, grad_ready, lib, stream_ptr
+from zookeeper_amd.ops._rows import DTYPE_CODES, guard, once_only, ptr, rows_of, use_kernels
+
+BLOCK = 32
+
+
+class Packed8:
+    """The 8-bit form of a tensor: ``codes`` int8 of its shape, ``scales`` uint8
+    with a last dimension of ``ceil(n / 32)``; a value is ``code * 2^(scale -
+    133)``, scale 255 stands for NaN.  ``dtype``: the packed tensor's type."""
+
+    __slots__ = ("codes", "scales", "dtype")
+
+    def __init__(self, codes: torch.Tensor, scales: torch.Tensor, dtype: torch.dtype):
+        want = (*codes.shape[:-1], -(-codes.shape[-1] // BLOCK)) if codes.dim() else None
+        if (codes.dtype != torch.int8 or scales.dtype != torch.uint8 or want is None
+                or tuple(scales.shape) != want or codes.device != scales.device
+                or not codes.is_contiguous() or not scales.is_contiguous()
+                or not dtype.is_floating_point):
+            raise ValueError(
+                "Packed8: expected contiguous int8 codes [..., n] and uint8 scales "
+                f"[..., ceil(n / {BLOCK})] on one device, got {codes.dtype} {tuple(codes.shape)} "
+                f"and {scales.dtype} {tuple(scales.shape)}")
+        self.codes, self.scales, self.dtype = codes, scales, dtype
+
+    @property
+    def shape(self) -> torch.Size:
+        return self.codes.shape
+
+    @property
+    def device(self) -> torch.device:
+        return self.codes.device
+
+    @property
+    def nbytes(self) -> int:
+        return self.codes.numel() + self.scales.numel()
+
+    def __repr__(self) -> str:
+        return f"Packed8(shape={tuple(self.shape)}, dtype={self.dtype}, device={self.device})"
+
+
+def _check_input(x: torch.Tensor, what: str) -> None:
+    if x.dim() == 0 or x.shape[-1] == 0:
+        raise ValueError(f"{what}: needs a non-empty last dimension, got {tuple(x.shape)}")
+
+
+def _empty_form(x):
+    codes = torch.empty(x.shape, dtype=torch.int8, device=x.device)
+    scales = torch.empty((*x.shape[:-1], -(-x.shape[-1] // BLOCK)), dtype=torch.uint8,
+                         device=x.device)
+    return codes, scales
+
+
+# --- the definitions in PyTorch (host tensors) --------------------------------
+
+def _steps(scales):
+    """2^(scale - 133) of each block, fp32; NaN for 255."""
+    s = scales.to(torch.int32)
+    step = ((s - 6).clamp_min(1) << 23).view(torch.float32)
+    return torch.where(s == 255, torch.full_like(step, float("nan")), step)
+
+
+def _pack_plain(x):
+    n = x.shape[-1]
+    v = F.pad(x.detach().float(), (0, -n % BLOCK)).unflatten(-1, (-1, BLOCK))
+    top = v.abs().amax(-1)  # NaN if the block holds one
+    fine = torch.isfinite(top)
+    top = torch.where(fine, top, torch.ones_like(top))
+    e = (top.contiguous().view(torch.int32) >> 23).clamp_min(7)
+    inv = ((260 - e) << 23).view(torch.float32)
+    e = e + (((top * inv).round() >= 128) & (e < 254)).to(torch.int32)
+    inv = ((260 - e) << 23).view(torch.float32)
+    codes = (v * inv.unsqueeze(-1)).round().clamp(-127, 127)
+    codes = torch.where(fine.unsqueeze(-1), codes, torch.zeros_like(codes))
+    e = torch.where(fine, e, torch.full_like(e, 255))
+    return (codes.to(torch.int8).flatten(-2)[..., :n].contiguous(), e.to(torch.uint8).contiguous())
+
+
+def _unpack_plain(codes, scales, dtype):
+    n = codes.shape[-1]
+    step = _steps(scales).repeat_interleave(BLOCK, -1)[..., :n]
+    return (codes.float() * step).to(dtype)
+
+
+def _gelu_slope(k):
+    return (0.5 * torch.erfc(k * -math.sqrt(0.5))
+            + k * torch.exp(-0.5 * k * k) * (1 / math.sqrt(2 * math.pi)))
+
+
+# --- pack / unpack --------------------------------------------------------------
+
+def pack8(x: torch.Tensor) -> Packed8:
+    """The 8-bit form of ``x`` (fp32, bf16 or fp16 on the GPU; any leading shape
+    and row stride).  Not differentiable: the form is what a backward keeps."""
+    _check_input(x, "pack8")
+    if not use_kernels(x, "pack8"):
+        return Packed8(*_pack_plain(x), x.dtype)
+    codes, scales = _empty_form(x)
+    x2, rows, stride = rows_of(x)
+    with guard(x):
+        check(lib().zk_pack8(x2.data_ptr(), codes.data_ptr(), scales.data_ptr(), rows,
+                             x.shape[-1], stride, DTYPE_CODES[x.dtype], stream_ptr(x.device)),
+              "zk_pack8")
+    return Packed8(codes, scales, x.dtype)
+
+
+def unpack8(kept: Packed8, dtype: Optional[torch.dtype] = None) -> torch.Tensor:
+    """The values that ``kept`` stands for, in ``dtype`` (default: the packed
+    tensor's type).  Exact in bf16 and fp32."""
+    dtype = kept.dtype if dtype is None else dtype
+    out = torch.empty(kept.shape, dtype=dtype, device=kept.device)
+    if not use_kernels(out, "unpack8"):
+        return _unpack_plain(kept.codes, kept.scales, dtype)
+    n = kept.shape[-1]
+    with guard(out):
+        check(lib().zk_unpack8(kept.codes.data_ptr(), kept.scales.data_ptr(), out.data_ptr(),
+                               out.numel() // n, n, DTYPE_CODES[dtype], stream_ptr(out.device)),
+              "zk_unpack8")
+    return out
+
+
+# --- GELU -------------------------------------------------------------------------
+
+def _gelu_forward(x, keep: bool):
+    y = torch.empty(x.shape, dtype=x.dtype, device=x.device)
+    codes, scales = _empty_form(x) if keep else (None, None)
+    x2, rows, stride = rows_of(x)
+    with guard(x):
+        check(lib().zk_gelu8_fwd(x2.data_ptr(), y.data_ptr(), ptr(codes), ptr(scales), rows,
+                                 x.shape[-1], stride, DTYPE_CODES[x.dtype],
+                                 stream_ptr(x.device)), "zk_gelu8_fwd")
+    return y, codes, scales
+
+
+class _Gelu8Fn(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, x, native):
+        if native:
+            y, codes, scales = _gelu_forward(x, True)
+        else:
+            y = F.gelu(x)
+            codes, scales = _pack_plain(x)
+        ctx.save_for_backward(codes, scales)
+        ctx.native = native
+        return y
+
+    @staticmethod
+    def backward(ctx, dy):
+        once_only("gelu8")
+        codes, scales = ctx.saved_tensors
+        if not ctx.native:
+            k = _unpack_plain(codes, scales, torch.float32).to(
+                torch.float64 if dy.dtype == torch.float64 else torch.float32)
+            return (dy.to(k.dtype) * _gelu_slope(k)).to(dy.dtype), None
+        dx = torch.empty(dy.shape, dtype=dy.dtype, device=dy.device)
+        dy2, rows, stride = rows_of(dy)
+        with guard(dy):
+            check(lib().zk_gelu8_bwd(dy2.data_ptr(), codes.data_ptr(), scales.data_ptr(),
+                                     dx.data_ptr(), rows, dy.shape[-1], stride,
+                                     DTYPE_CODES[dy.dtype], stream_ptr(dy.device)),
+                  "zk_gelu8_bwd")
+        return dx, None
+
+
+def gelu8(x: torch.Tensor) -> torch.Tensor:
+    """``x * Phi(x)``; the input is kept in 8 bits for the backward (nothing is
+    kept when no gradient is wanted).  See the module docstring."""
+    _check_input(x, "gelu8")
+    native = use_kernels(x, "gelu8")
+    if x.requires_grad and torch.is_grad_enabled():
+        return _Gelu8Fn.apply(x, native)
+    return _gelu_forward(x, False)[0] if native else F.gelu(x)
+
+
+# --- dense ------------------------------------------------------------------------
+
+def _dense_grads(dy, codes, scales, want_w: bool, want_b: bool, dw=None, db=None):
+    """fp32 ``dw`` [N, K] and ``db`` [N] of ``dy`` [..., N] and the kept input
+    [..., K]; given ``dw`` / ``db`` buffers are added to."""
+    N, K = dy.shape[-1], codes.shape[-1]
+    dev = dy.device
+    dy2, rows, stride = rows_of(dy)
+    add = (1 if dw is not None else 0) | (2 if db is not None else 0)
+    new = torch.zeros if rows == 0 else torch.empty
+    if want_w and dw is None:
+        dw = new((N, K), dtype=torch.float32, device=dev)
+    if want_b and db is None:
+        db = new((N,), dtype=torch.float32, device=dev)
+    if rows == 0:
+        return dw, db
+    L = lib()
+    ws_bytes = L.zk_dense8_wgrad_ws_bytes(rows, N, K)
+    if ws_bytes < 0:
+        raise ValueError(f"dense8: sizes rows={rows}, outputs={N}, inputs={K} are not supported")
+    ws = torch.empty(max(ws_bytes // 4, 1), dtype=torch.float32, device=dev)
+    with guard(dy):
+        check(L.zk_dense8_wgrad(dy2.data_ptr(), codes.data_ptr(), scales.data_ptr(),
+                                dw.data_ptr(), ptr(db) if want_b else None, ws.data_ptr(),
+                                ws_bytes, rows, N, K, stride, DTYPE_CODES[dy.dtype], add,
+                                stream_ptr(dev)), "zk_dense8_wgrad")
+    return dw, db
+
+
+def dense8_grads(dy: torch.Tensor, kept: Packed8,
+                 bias: bool = True) -> Tuple[torch.Tensor, Optional[torch.Tensor]]:
+    """``(dw, db)`` of a dense layer ``y = x w^T + b`` in fp32: ``dw`` [N, K] =
+    ``dy^T x8`` and ``db`` [N] = the sum of ``dy`` over its rows (None without
+    ``bias``), from the output gradient ``dy`` [..., N] (fp32, bf16 or fp16, any
+    row stride) and the kept input [..., K].
+
+    bf16 gradients take one matrix product, fp16 and fp32 gradients two and
+    three (their exact bf16 terms); sums are fp32 in a fixed order."""
+    _check_input(dy, "dense8_grads")
+    if dy.shape[:-1] != kept.shape[:-1]:
+        raise ValueError(f"dense8_grads: rows differ: dy {tuple(dy.shape)}, "
+                         f"kept input {tuple(kept.shape)}")
+    if dy.device != kept.device:
+        raise ValueError(f"dense8_grads: dy on {dy.device}, the kept input on {kept.device}")
+    dy = dy.detach()
+    if use_kernels(dy, "dense8_grads"):
+        return _dense_grads(dy, kept.codes, kept.scales, True, bias)
+    d = dy.reshape(-1, dy.shape[-1]).float()
+    x = _unpack_plain(kept.codes, kept.scales, torch.float32).reshape(-1, kept.shape[-1])
+    return d.t() @ x, d.sum(0) if bias else None
+
+
+class _Dense8Fn(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, x, weight, bias):
+        w = weight.to(x.dtype)
+        y = F.linear(x, w, bias.to(x.dtype) if bias is not None else None)
+        codes = scales = None
+        if ctx.needs_input_grad[1]:
+            kept = pack8(x)
+            codes, scales = kept.codes, kept.scales
+        ctx.save_for_backward(codes, scales, weight)
+        ctx.weight_param, ctx.bias_param = weight, bias
+        return y
+
+    @staticmethod
+    def backward(ctx, dy):
+        once_only("dense8")
+        codes, scales, weight = ctx.saved_tensors
+        need_x, need_w, need_b = ctx.needs_input_grad
+        wp, bp = ctx.weight_param, ctx.bias_param
+        dx = torch.matmul(dy, weight.to(dy.dtype)) if need_x else None
+        dw = db = None
+        native = use_kernels(dy, "dense8")
+        dw_direct = direct_grad(wp) if need_w and native else None
+        db_direct = direct_grad(bp) if need_b and native else None
+        if need_w and native:
+            dw, db = _dense_grads(dy, codes, scales, True, need_b, dw_direct, db_direct)
+        elif need_w:
+            dw, db = dense8_grads(dy, Packed8(codes, scales, dy.dtype), need_b)
+        elif need_b:  # a frozen weight with a trainable bias
+            db = dy.reshape(-1, dy.shape[-1]).float().sum(0)
+            if db_direct is not None:
+                db_direct += db
+        if dw_direct is not None:
+            grad_ready(wp)
+            dw = None
+        elif dw is not None:
+            dw = dw.to(wp.dtype)
+        if db_direct is not None:
+            grad_ready(bp)
+            db = None
+        elif db is not None:
+            db = db.to(bp.dtype)
+        return dx, dw, db
+
+
+def dense8(x: torch.Tensor, weight: torch.Tensor,
+           bias: Optional[torch.Tensor] = None) -> torch.Tensor:
+    """``x weight^T + bias`` in ``x``'s type, its input kept in 8 bits for the
+    weight gradient; see the module docstring.  ``weight`` [N, K], ``bias`` [N]
+    of any floating type (their gradients have it; flat fp32 gradient buffers
+    are accumulated into directly)."""
+    _check_input(x, "dense8")
+    if weight.dim() != 2 or weight.shape[1] != x.shape[-1] or weight.shape[0] == 0:
+        raise ValueError(f"dense8: weight of shape (outputs, {x.shape[-1]}) expected, "
+                         f"got {tuple(weight.shape)}")
+    if bias is not None and tuple(bias.shape) != (weight.shape[0],):
+        raise ValueError(f"dense8: bias of shape ({weight.shape[0]},) expected, "
+                         f"got {tuple(bias.shape)}")
+    for name, p in (("weight", weight), ("bias", bias)):
+        if p is not None and (p.device != x.device or not p.is_floating_point()):
+            raise ValueError(f"dense8: {name} must be a floating-point tensor on {x.device}, "
+                             f"got {p.dtype} on {p.device}")
+    use_kernels(x, "dense8")
+    if torch.is_grad_enabled() and (x.requires_grad or weight.requires_grad
+                                    or (bias is not None and bias.requires_grad)):
+        return _Dense8Fn.apply(x, weight, bias)
+    return F.linear(x, weight.to(x.dtype), bias.to(x.dtype) if bias is not None else None)
