@@ -217,6 +217,35 @@ def test_dense_gradients(rows, outs, cols, dt):
     assert again[1] is None and torch.equal(again[0], dw)
 
 
+WIDE = [(64, 1, 64), (65, 5, 70), (130, 300, 100), (257, 257, 257), (700, 1, 600),
+        (1000, 515, 1001), (2049, 384, 640), (4096, 1024, 512), (64, 2048, 1536),
+        (1300, 1000, 512), (9001, 72, 96), (3333, 260, 67)]
+
+
+@pytest.mark.parametrize("variant", [0, 1])
+@pytest.mark.parametrize("dt", DTYPES)
+@pytest.mark.parametrize("rows,outs,cols", WIDE)
+def test_dense_gradients_of_each_kernel(rows, outs, cols, dt, variant):
+    from zookeeper_amd.ops import pack8
+    from zookeeper_amd.ops.act8 import _dense_grads
+
+    torch.manual_seed(rows + outs + cols)
+    x = torch.randn(rows, cols, device="cuda").to(dt)
+    dy = torch.randn(rows, outs, device="cuda").to(dt)
+    kept = pack8(x)
+    h, d = _held(x), dy.double()
+    tol = (rows + 16) * 2.0 ** -23
+    want, mag = d.t() @ h, d.abs().t() @ h.abs()
+    wb, mb = d.sum(0), d.abs().sum(0)
+    dw, db = _dense_grads(dy, kept.codes, kept.scales, True, variant=variant)
+    assert ((dw.double() - want).abs() <= tol * mag + 1e-30).all()
+    assert ((db.double() - wb).abs() <= tol * mb + 1e-30).all()
+    # added to buffers, and again: the same bits
+    w2, b2 = torch.ones_like(dw), torch.full_like(db, 2.0)
+    _dense_grads(dy, kept.codes, kept.scales, True, w2, b2, variant=variant)
+    assert torch.equal(w2, dw + 1) and torch.equal(b2, db + 2)
+
+
 def test_dense_rows_with_gaps_and_special_values():
     from zookeeper_amd.ops import dense8_grads, pack8
 

@@ -21,6 +21,8 @@
 
 namespace {
 
+typedef unsigned long long u64_t;
+
 constexpr int kNT = 256;
 
 // max over the quad of lanes that shares a 32-value block
@@ -234,7 +236,8 @@ struct D8Args {
   const uint8_t* scales;  // [M][kb]
   float* dw;              // [N][K]
   float* db;              // [N] or null
-  float* slab;            // [splits][N][K], then [splits * ktiles][N] for db
+  float* slab;            // [splits][N][K] (several splits)
+  float* part;            // [splits * ktiles][N]: db's parts
   long long dys;
   long long M;
   int N, K, kb, ntiles, ktiles, splits, add;
@@ -246,14 +249,15 @@ __device__ __forceinline__ f32x4 mma16(const uint4& a, const uint4& b, const f32
                                                  __builtin_bit_cast(bf16x8, b), c, 0, 0, 0);
 }
 
-// 8 consecutive m of column c0 + (lane & 15) from a swizzled [m][128] bf16 plane:
+// 8 consecutive m of column c0 + (lane & 15) from a swizzled [m][RB / 2] bf16 plane:
 // lane l: m = 8 (l >> 4) ..
+template <int RB>
 __device__ __forceinline__ uint4 col_frag(const unsigned char* plane, int c0, int lane) {
   const int g = lane >> 4, i = lane & 15, q = i >> 2, p = i & 3;
   const int r0 = 8 * g + q, r1 = r0 + 4;
   const int slot = (c0 >> 3) | (p >> 1), inner = (p & 1) * 8;
-  const int o0 = r0 * 256 + ((slot ^ tr_swz<256>(r0)) << 4) + inner;
-  const int o1 = r1 * 256 + ((slot ^ tr_swz<256>(r1)) << 4) + inner;
+  const int o0 = r0 * RB + ((slot ^ tr_swz<RB>(r0)) << 4) + inner;
+  const int o1 = r1 * RB + ((slot ^ tr_swz<RB>(r1)) << 4) + inner;
   typedef __attribute__((address_space(3))) s16x4 lds_s16x4;
   const s16x4 lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16(
       (lds_s16x4*)(uintptr_t)(const __attribute__((address_space(3))) void*)(plane + o0));
@@ -385,13 +389,13 @@ __global__ __launch_bounds__(kNT, 2) void dense8_wgrad_kernel(D8Args a) {
     const unsigned char* buf = smem + (s & 1) * BUF;
     uint4 x[4];
 #pragma unroll
-    for (int j = 0; j < 4; ++j) x[j] = col_frag(buf + TERMS * kPlane, wk * 64 + j * 16, lane);
+    for (int j = 0; j < 4; ++j) x[j] = col_frag<256>(buf + TERMS * kPlane, wk * 64 + j * 16, lane);
     const bool sum = a.db && wk == 0 && s % a.ktiles == kt;
 #pragma unroll
     for (int t = 0; t < TERMS; ++t) {
       uint4 d[4];
 #pragma unroll
-      for (int i = 0; i < 4; ++i) d[i] = col_frag(buf + t * kPlane, wn * 64 + i * 16, lane);
+      for (int i = 0; i < 4; ++i) d[i] = col_frag<256>(buf + t * kPlane, wn * 64 + i * 16, lane);
 #pragma unroll
       for (int i = 0; i < 4; ++i)
 #pragma unroll
@@ -422,8 +426,7 @@ __global__ __launch_bounds__(kNT, 2) void dense8_wgrad_kernel(D8Args a) {
       }
     }
   if (a.db && wk == 0 && (lane & 15) == 0) {
-    float* part = a.slab + (direct ? 0 : (long long)a.splits * a.N * a.K) +
-                  ((long long)split * a.ktiles + kt) * a.N;
+    float* part = a.part + ((long long)split * a.ktiles + kt) * a.N;
 #pragma unroll
     for (int i = 0; i < 4; ++i)
 #pragma unroll
@@ -431,6 +434,315 @@ __global__ __launch_bounds__(kNT, 2) void dense8_wgrad_kernel(D8Args a) {
         const int n = n0 + wn * 64 + i * 16 + 4 * (lane >> 4) + e;
         if (n < a.N) part[n] = bacc[i][e];
       }
+  }
+}
+
+// ---------------------------------------------------------------------------
+// The same product for large sizes: a block of 8 waves owns a 256 x 256 tile and
+// walks 64 rows a step in two halves of 32.  dy rows go to LDS by LDS-DMA, one
+// step ahead; codes go through registers, two steps ahead of their use, are
+// decoded between the matrix instructions of the step before and stored as bf16
+// rows.  Two buffers of 64 KB.  One wave holds 128 x 64 of the tile, 32
+// accumulators of 16 x 16.
+//
+// Per step and half: the fragments of the other row half of dy are read while
+// this half's products run; every barrier is preceded by the LDS waits of the
+// wave's own reads and writes.  Loads return in order, so a code whose value has
+// arrived proves that the dy pieces asked for before it have landed too; the
+// explicit vmcnt waits count the instructions behind the piece that is needed (2
+// per dy piece, 4 per code piece).  Behind the last row both kinds read valid
+// stand-ins, so the counts never change.
+//
+// dy needs whole 16-byte chunks (N and the row stride multiples of 8, 16-byte
+// base).  Any other dy, and fp16 / fp32, is first cut into its bf16 terms,
+// [term][M][N8], and the product runs over the terms' rows one after the other
+// (virtual row r: kept row r mod M).
+// ---------------------------------------------------------------------------
+constexpr int kW = 256;                 // tile edge
+constexpr int kWNT = 512;               // threads
+constexpr int kWPiece = 32 * kW * 2;    // 32 rows of 512 B
+constexpr int kWBuf = 4 * kWPiece;      // dy halves 0 and 1, x halves 0 and 1
+
+__device__ __attribute__((aligned(512))) uint4 g_a8_zero[32];  // 512 B of zeros
+
+struct D8WideArgs {
+  const uint16_t* dy;     // [R][dys] bf16, R = terms * M
+  const int8_t* codes;    // [M][K]
+  const uint8_t* scales;  // [M][kb]
+  float* dw;
+  float* db;
+  float* slab;
+  float* part;
+  long long dys, rps;  // rps: virtual rows of a split (multiple of 64)
+  int M, R, N, K, kb, ntiles, ktiles, splits, add;
+};
+
+// 16 bytes per lane to LDS address lds (wave-uniform) + 16 * lane
+__device__ __forceinline__ void dma16(const void* src, uint32_t lds) {
+  asm volatile("s_mov_b32 m0, %1\n\tglobal_load_lds_dwordx4 %0, off" ::"v"(src), "s"(lds)
+               : "m0", "memory");
+}
+
+__device__ __forceinline__ void lds_barrier() {
+  asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory");
+}
+
+__global__ __launch_bounds__(kWNT, 2) void dense8_wide_kernel(D8WideArgs a) {
+  extern __shared__ __attribute__((aligned(1024))) unsigned char smem[];
+  typedef __attribute__((address_space(3))) unsigned char lds_u8;
+  typedef __attribute__((address_space(3))) s16x4 lds_s16x4;
+  typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
+  typedef __attribute__((address_space(3))) u32x4 lds_u128;
+  const uint32_t lds0 = (uint32_t)(uintptr_t)(lds_u8*)smem;
+  const int tid = threadIdx.x, lane = tid & 63;
+  const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const int wn = wave >> 2, wk = wave & 3;
+  const int L = xcd_linear(blockIdx.x, gridDim.x);
+  const int tiles = a.ntiles * a.ktiles;
+  const int split = L / tiles, tile = L - split * tiles;
+  const int kt = tile % a.ktiles, nt = tile / a.ktiles;
+  const int n0 = nt * kW, k0 = kt * kW;
+  // R < 2^31 - 256: the steps that run ahead of the last row fit too
+  const int r0 = (int)(split * a.rps), r1 = (int)min((long long)a.R, r0 + a.rps);
+  const int steps = (r1 - r0 + 63) >> 6;
+
+  // dy: instruction i of wave w fills piece rows (8 i + w) * 2 + (lane >> 5); LDS slot
+  // lane & 31 holds the row's 16-byte chunk (lane & 31) ^ tr_swz(row).  Chunks behind N
+  // are the tile's first one (their rows of dW are not stored).
+  const int arow = wave * 2 + (lane >> 5);  // i = 1: + 16, the same swizzle
+  const int chunk = (lane & 31) ^ tr_swz<512>(arow);
+  const int acol = n0 + chunk * 8 < a.N ? chunk * 16 : 0;
+  const unsigned char* dyb = reinterpret_cast<const unsigned char*>(a.dy) + n0 * 2LL + acol;
+  const unsigned char* zero = reinterpret_cast<const unsigned char*>(g_a8_zero) + chunk * 16;
+  const uint32_t dyrow = (uint32_t)a.dys * 2u;
+  auto issue = [&](int s, int h) {
+    const uint32_t dst = lds0 + (s & 1) * kWBuf + h * kWPiece + wave * 1024;
+    const int rb = r0 + s * 64 + h * 32 + arow;
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+      const int r = rb + 16 * i;
+      dma16(r < r1 ? dyb + (u64_t)(uint32_t)r * dyrow : zero, dst + i * 8192);
+    }
+  };
+
+  // codes: 8 of columns 8 (tid & 31) of rows tid >> 5 and + 16 of a half.  A chunk that K
+  // cuts is read from the row's last 8 and moved down; columns behind K: any valid place.
+  // Rows behind the split: the first one (put() makes them zeros).
+  const int crow = tid >> 5, col = k0 + (tid & 31) * 8;
+  const int cc = col >= a.K ? 0 : min(col, a.K - 8);
+  const int back = col >= a.K ? 0 : 8 * (col - cc);
+  const int8_t* cp = a.codes + cc;
+  const uint8_t* sp = a.scales + ((col >= a.K ? 0 : col) >> 5);
+  struct Codes {
+    Bytes8 w[2];
+    uint32_t e[2];
+  };
+  auto fetch = [&](Codes& c, int s, int h) {
+    const int rb = r0 + s * 64 + h * 32;  // uniform
+    int mb = rb >= a.M ? rb - a.M : rb;   // row in its term: at most two terms back
+    mb = mb >= a.M ? mb - a.M : mb;
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+      int m = mb + crow + 16 * i;
+      m = m >= a.M ? m - a.M : m;  // the next term starts inside the piece (M >= 64)
+      m = rb + crow + 16 * i < r1 ? m : 0;
+      c.w[i] = *reinterpret_cast<const Bytes8*>(cp + (u64_t)(uint32_t)m * (uint32_t)a.K);
+      c.e[i] = sp[(u64_t)(uint32_t)m * (uint32_t)a.kb];
+    }
+  };
+  // the other 16 rows of a half have the same swizzle
+  uint32_t xput = crow * 512 + (((tid & 31) ^ tr_swz<512>(crow)) << 4);
+  auto put = [&](const Codes& c, int s, int h) {
+    const uint32_t at = lds0 + (xput ^ ((s & 1) * kWBuf));
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+      const bool live = r0 + s * 64 + h * 32 + 16 * i + crow < r1;
+      const float st = live ? step_of(c.e[i]) : 0.f;
+      const float off = -128.f * st;
+      const u64_t v = (((u64_t)c.w[i][1] << 32) | c.w[i][0]) >> back;
+      const uint32_t b[2] = {(uint32_t)v ^ 0x80808080u, (uint32_t)(v >> 32) ^ 0x80808080u};
+      uint32_t o[4];
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        // code + 128 as an unsigned byte: the conversion picks the byte itself
+        const uint32_t w = b[j >> 1];
+        const float x = (float)((w >> (16 * (j & 1))) & 0xffu);
+        const float y = (float)((w >> (16 * (j & 1) + 8)) & 0xffu);
+        o[j] = zk::pack_bf16x2(__builtin_fmaf(x, st, off), __builtin_fmaf(y, st, off));
+      }
+      *(lds_u128*)(uintptr_t)(at + (2 + h) * kWPiece + i * 8192) = u32x4{o[0], o[1], o[2], o[3]};
+    }
+  };
+
+  f32x4 acc[8][4], bacc[2];
+#pragma unroll
+  for (int i = 0; i < 8; ++i)
+#pragma unroll
+    for (int j = 0; j < 4; ++j) acc[i][j] = f32x4{0.f, 0.f, 0.f, 0.f};
+  bacc[0] = bacc[1] = f32x4{0.f, 0.f, 0.f, 0.f};
+  const uint4 ones = {0x3F803F80u, 0x3F803F80u, 0x3F803F80u, 0x3F803F80u};
+  uint4 d1[4], d2[4], x1[4], x2[4];
+  // A fragment's byte address is (lane part) ^ (column block part): row, swizzled
+  // chunk and buffer occupy separate bits.  Rows + 4: + 2048 and the chunk's lowest bit
+  // flipped.  Recomputed at each read (one xor): kept in registers the 48
+  // addresses would spill.
+  const int q4 = (lane & 15) >> 2, p4 = lane & 3, frow = 8 * (lane >> 4) + q4;
+  const uint32_t f0 = frow * 512 + (((p4 >> 1) ^ tr_swz<512>(frow)) << 4) + (p4 & 1) * 8;
+  uint32_t fd = f0 ^ (wn * 256), fx = f0 ^ (wk * 128);
+  auto frag = [&](uint32_t l, uint32_t block, uint32_t piece) {
+    const uint32_t at = lds0 + piece + (l ^ block);
+    const uint32_t at4 = lds0 + piece + 2048 + (l ^ block ^ 16u);
+    const s16x4 lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4*)(uintptr_t)at);
+    const s16x4 hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4*)(uintptr_t)at4);
+    const s16x8 v = {lo[0], lo[1], lo[2], lo[3], hi[0], hi[1], hi[2], hi[3]};
+    return __builtin_bit_cast(uint4, v);
+  };
+  auto readD = [&](uint4 (&d)[4], int s, int h, int mh) {
+    uint32_t l = fd ^ ((s & 1) * kWBuf);
+    asm volatile("" : "+v"(l));
+#pragma unroll
+    for (int i = 0; i < 4; ++i) d[i] = frag(l, mh * 128 + i * 32, h * kWPiece);
+  };
+  auto readX = [&](uint4 (&d)[4], int s, int h) {
+    uint32_t l = fx ^ ((s & 1) * kWBuf);
+    asm volatile("" : "+v"(l));
+#pragma unroll
+    for (int j = 0; j < 4; ++j) d[j] = frag(l, j * 32, (2 + h) * kWPiece);
+  };
+  auto mma = [&](const uint4 (&d)[4], const uint4 (&x)[4], int mh) {
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+#pragma unroll
+      for (int j = 0; j < 4; ++j) acc[mh * 4 + i][j] = mma16(d[i], x[j], acc[mh * 4 + i][j]);
+  };
+  // db: the four waves with the same dy columns take a quarter of their fragments each
+  auto sums = [&](const uint4 (&d)[4], int mh) {
+    if ((wk >> 1) != mh) return;
+    if (wk & 1) {
+      bacc[0] = mma16(d[2], ones, bacc[0]);
+      bacc[1] = mma16(d[3], ones, bacc[1]);
+    } else {
+      bacc[0] = mma16(d[0], ones, bacc[0]);
+      bacc[1] = mma16(d[1], ones, bacc[1]);
+    }
+  };
+
+  Codes c0, c1;
+  issue(0, 0);
+  fetch(c0, 0, 0);
+  fetch(c1, 0, 1);
+  put(c0, 0, 0);
+  put(c1, 0, 1);
+  fetch(c0, 1, 0);
+  issue(0, 1);
+  fetch(c1, 1, 1);
+  wait_vmcnt<0>();
+  lds_barrier();
+  readD(d1, 0, 0, 0);
+  readX(x1, 0, 0);
+  for (int s = 0; s < steps; ++s) {
+    const bool sum = a.db && s % a.ktiles == kt;  // uniform
+    // half 0, rows of dy's first columns
+    readD(d2, s, 0, 1);
+    __builtin_amdgcn_sched_barrier(0);
+    put(c0, s + 1, 0);
+    mma(d1, x1, 0);
+#pragma unroll
+    for (int i = 0; i < 16; ++i) {
+      __builtin_amdgcn_sched_group_barrier(0x008, 1, 0);
+      __builtin_amdgcn_sched_group_barrier(0x002, 5, 0);
+    }
+    __builtin_amdgcn_sched_barrier(0);
+    if (sum) sums(d1, 0);
+    issue(s + 1, 0);
+    fetch(c0, s + 2, 0);
+    __builtin_amdgcn_sched_barrier(0);
+    wait_vmcnt<10>();  // dy half 1 of this step; behind it: codes, dy, codes
+    lds_barrier();
+    readD(d1, s, 1, 0);
+    readX(x2, s, 1);
+    __builtin_amdgcn_sched_barrier(0);
+    mma(d2, x1, 1);
+    if (sum) sums(d2, 1);
+    __builtin_amdgcn_sched_barrier(0);
+    // half 1
+    readD(d2, s, 1, 1);
+    __builtin_amdgcn_sched_barrier(0);
+    put(c1, s + 1, 1);
+    mma(d1, x2, 0);
+#pragma unroll
+    for (int i = 0; i < 16; ++i) {
+      __builtin_amdgcn_sched_group_barrier(0x008, 1, 0);
+      __builtin_amdgcn_sched_group_barrier(0x002, 5, 0);
+    }
+    __builtin_amdgcn_sched_barrier(0);
+    if (sum) sums(d1, 0);
+    issue(s + 1, 1);
+    fetch(c1, s + 2, 1);
+    __builtin_amdgcn_sched_barrier(0);
+    wait_vmcnt<10>();  // dy half 0 of the next step
+    lds_barrier();
+    readD(d1, s + 1, 0, 0);
+    readX(x1, s + 1, 0);
+    __builtin_amdgcn_sched_barrier(0);
+    mma(d2, x2, 1);
+    if (sum) sums(d2, 1);
+    __builtin_amdgcn_sched_barrier(0);
+  }
+  wait_vmcnt<0>();  // no LDS-DMA may outlive the block
+
+  const bool direct = a.splits == 1;
+  float* out = direct ? a.dw : a.slab + (long long)split * a.N * a.K;
+  const bool add = direct && (a.add & 1);
+#pragma unroll
+  for (int i = 0; i < 8; ++i)
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+      const int n = n0 + wn * 128 + i * 16 + 4 * (lane >> 4) + e;
+      if (n >= a.N) continue;
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        const int k = k0 + wk * 64 + j * 16 + (lane & 15);
+        if (k < a.K) {
+          float* o = out + (long long)n * a.K + k;
+          *o = add ? *o + acc[i][j][e] : acc[i][j][e];
+        }
+      }
+    }
+  if (a.db && (lane & 15) == 0) {
+    float* part = a.part + ((long long)split * a.ktiles + kt) * a.N;
+#pragma unroll
+    for (int i = 0; i < 2; ++i)
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        const int n = n0 + wn * 128 + (2 * wk + i) * 16 + 4 * (lane >> 4) + e;
+        if (n < a.N) part[n] = bacc[i][e];
+      }
+  }
+}
+
+// dy [M][dys] -> its bf16 terms [TERMS][M][N8], columns behind N zero
+template <int DT>
+__global__ __launch_bounds__(kNT) void dense8_terms_kernel(const void* dy, long long dys,
+                                                           long long M, int N, int N8,
+                                                           uint16_t* out) {
+  constexpr int TERMS = DT == 1 ? 1 : DT == 2 ? 2 : 3;
+  typedef typename Elem<DT>::raw raw;
+  const int chunks = N8 >> 3;
+  const long long total = M * chunks, step = (long long)gridDim.x * kNT;
+  for (long long id = (long long)blockIdx.x * kNT + threadIdx.x; id < total; id += step) {
+    const long long m = id / chunks;
+    const int c = (int)(id - m * chunks) * 8;
+    float f[8];
+    load8_n<DT>(reinterpret_cast<const raw*>(dy) + m * dys + c, N - c, 0.f, f);
+#pragma unroll
+    for (int t = 0; t < TERMS; ++t) {
+      uint32_t h[8];
+#pragma unroll
+      for (int j = 0; j < 8; ++j) h[j] = cut_term(f[j]);
+      *reinterpret_cast<uint4*>(out + ((long long)t * M + m) * N8 + c) =
+          uint4{h[0] | (h[1] << 16), h[2] | (h[3] << 16), h[4] | (h[5] << 16), h[6] | (h[7] << 16)};
+    }
   }
 }
 
@@ -454,31 +766,80 @@ __global__ __launch_bounds__(1024) void dense8_sum_kernel(const float* __restric
   }
 }
 
+// Sizes and workspace of one call.  wide: the 256 x 256 kernel.
 struct D8Plan {
-  int ntiles, ktiles, splits;
-  long long mps, slab, bytes;
+  bool wide, terms;       // terms: dy is cut into its bf16 terms first
+  int ntiles, ktiles, splits, N8;
+  long long rps;          // rows (wide: virtual rows) of a split
+  long long slab, parts;  // floats
+  long long bytes;
 };
 
-// Two blocks per CU, at least 256 rows per split.
-D8Plan dense8_plan(long long M, int N, int K) {
-  D8Plan p;
-  p.ntiles = (N + kT - 1) / kT;
-  p.ktiles = (K + kT - 1) / kT;
+D8Plan dense8_plan(long long M, int N, int K, int dt, long long dys, bool aligned, int variant) {
+  D8Plan p{};
+  // Measured per call, bf16: 2048 x 256 x 256 19 us (128) / 33 us (256), 4096 x 768 x 768
+  // 60 / 53, 16384 x 1024 x 1024 123 / 92, 16384 x 4096 x 4096 1534 / 641.
+  p.wide = variant == 1 || (variant < 0 && M >= 64 && N >= 128 && K >= 128 &&
+                            (double)M * N * K >= 2147483648.0);
+  const int T = p.wide ? kW : kT;
+  p.ntiles = (N + T - 1) / T;
+  p.ktiles = (K + T - 1) / T;
   const long long tiles = (long long)p.ntiles * p.ktiles;
-  long long s = (512 + tiles - 1) / tiles;
-  const long long most = (M + 255) / 256;
-  if (s > most) s = most;
-  if (s < 1) s = 1;
-  p.mps = ((M + s - 1) / s + kMS - 1) / kMS * kMS;
-  p.splits = (int)((M + p.mps - 1) / p.mps);
+  p.N8 = (N + 7) & ~7;
+  p.terms = p.wide && (dt != 1 || !aligned || N != p.N8 || (dys & 7));
+  const int terms = dt == 1 ? 1 : dt == 2 ? 2 : 3;
+  long long s = 1;
+  if (p.wide) {
+    // one block per CU and about a microsecond per step: the split that takes the fewest
+    // rounds of steps (12 more per block for its start and end) and slab bytes
+    const long long R = terms * M;
+    double best = 1e30;
+    for (long long c = 1; c <= 64 && (c == 1 || R / c >= 512); ++c) {
+      const double rounds = (double)((tiles * c + 255) / 256);
+      const double cost = rounds * ((double)(R / c) / 64 + 12) +
+                          (c > 1 ? 8e-6 / 5 * (double)c * N * K + 5 : 0);
+      if (cost < best) {
+        best = cost;
+        s = c;
+      }
+    }
+    p.rps = ((R + s - 1) / s + 63) / 64 * 64;
+    p.splits = (int)((R + p.rps - 1) / p.rps);
+  } else {
+    // two blocks per CU, at least 256 rows per split
+    s = (512 + tiles - 1) / tiles;
+    const long long most = (M + 255) / 256;
+    if (s > most) s = most;
+    if (s < 1) s = 1;
+    p.rps = ((M + s - 1) / s + kMS - 1) / kMS * kMS;
+    p.splits = (int)((M + p.rps - 1) / p.rps);
+  }
   p.slab = p.splits > 1 ? (long long)p.splits * N * K : 0;
-  p.bytes = 4 * (p.slab + (long long)p.splits * p.ktiles * N);
+  p.parts = (long long)p.splits * p.ktiles * N;
+  p.slab = (p.slab + 3) & ~3LL;
+  p.parts = (p.parts + 3) & ~3LL;  // the terms start 16-byte aligned
+  p.bytes = 4 * (p.slab + p.parts) + (p.terms ? 2LL * terms * M * p.N8 : 0);
   return p;
 }
 
-bool dense8_ok(long long M, int N, int K) {
-  return M >= 1 && N >= 1 && K >= 1 && M < (1LL << 31) && N < (1 << 24) && K < (1 << 24) &&
+bool dense8_ok(long long M, int N, int K, long long dys) {
+  return M >= 1 && N >= 1 && K >= 1 && M < (1LL << 29) && N < (1 << 24) && K < (1 << 24) &&
+         dys >= 0 && dys < (1 << 24) &&
          ((N + kT - 1LL) / kT) * ((K + kT - 1LL) / kT) < (1 << 20);
+}
+
+bool g_wide_attr = false;
+
+int dense8_wide_launch(const D8WideArgs& a, hipStream_t st) {
+  if (!g_wide_attr) {
+    const hipError_t e = hipFuncSetAttribute((const void*)dense8_wide_kernel,
+                                             hipFuncAttributeMaxDynamicSharedMemorySize, 2 * kWBuf);
+    if (e != hipSuccess) return (int)e;
+    g_wide_attr = true;
+  }
+  hipLaunchKernelGGL(dense8_wide_kernel, dim3((unsigned)(a.ntiles * a.ktiles * a.splits)),
+                     dim3(kWNT), 2 * kWBuf, st, a);
+  return (int)hipGetLastError();
 }
 
 }  // namespace
@@ -510,33 +871,67 @@ ZK_EXPORT int zk_gelu8_bwd(const void* dy, const void* codes, const void* scales
                                dys, dt, st);
 }
 
-// Workspace bytes of zk_dense8_wgrad, or -1 for sizes it does not take.
-ZK_EXPORT long long zk_dense8_wgrad_ws_bytes(long long M, int N, int K) {
-  return dense8_ok(M, N, K) ? dense8_plan(M, N, K).bytes : -1;
+// Workspace bytes of zk_dense8_wgrad for the same arguments (aligned: dy starts on
+// 16 bytes), or -1 for sizes it does not take.
+ZK_EXPORT long long zk_dense8_wgrad_ws_bytes(long long M, int N, int K, long long dys, int dt,
+                                             int aligned, int variant) {
+  if (!dense8_ok(M, N, K, dys) || dt < 0 || dt > 2 || variant > 1 ||
+      (variant == 1 && (M < 64 || K < 64)))
+    return -1;
+  return dense8_plan(M, N, K, dt, dys, aligned != 0, variant).bytes;
 }
 
 // dw [N][K] and db [N] (or null), fp32, from dy [M][dys] and the kept input
 // [M][K].  add: bit 0 dw, bit 1 db are accumulated into instead of written.
+// variant: 0 the 128 x 128 kernel, 1 the 256 x 256 one (M, K >= 64), -1 by size.
 ZK_EXPORT int zk_dense8_wgrad(const void* dy, const void* codes, const void* scales, void* dw,
                               void* db, void* ws, long long ws_bytes, long long M, int N, int K,
-                              long long dys, int dt, int add, hipStream_t st) {
-  if (!dense8_ok(M, N, K) || dys < 0 || dt < 0 || dt > 2) return (int)hipErrorInvalidValue;
-  const D8Plan p = dense8_plan(M, N, K);
-  if (!ws || ws_bytes < p.bytes) return (int)hipErrorInvalidValue;
-  D8Args a{dy, (const int8_t*)codes, (const uint8_t*)scales, (float*)dw, (float*)db, (float*)ws,
-           dys, M, N, K, (K + 31) / 32, p.ntiles, p.ktiles, p.splits, add, p.mps};
-  const dim3 g((unsigned)((long long)p.ntiles * p.ktiles * p.splits));
-  if (dt == 0) hipLaunchKernelGGL(dense8_wgrad_kernel<0>, g, dim3(kNT), 0, st, a);
-  if (dt == 1) hipLaunchKernelGGL(dense8_wgrad_kernel<1>, g, dim3(kNT), 0, st, a);
-  if (dt == 2) hipLaunchKernelGGL(dense8_wgrad_kernel<2>, g, dim3(kNT), 0, st, a);
-  ZK_CHECK_LAUNCH();
+                              long long dys, int dt, int add, int variant, hipStream_t st) {
+  const bool aligned = ((uintptr_t)dy & 15) == 0;
+  const long long need = zk_dense8_wgrad_ws_bytes(M, N, K, dys, dt, aligned, variant);
+  if (need < 0 || (need > 0 && !ws) || ws_bytes < need || ((uintptr_t)ws & 15))
+    return (int)hipErrorInvalidValue;
+  const D8Plan p = dense8_plan(M, N, K, dt, dys, aligned, variant);
+  const int kb = (K + 31) / 32;
+  float* const slab = (float*)ws;
+  if (p.wide) {
+    const int terms = dt == 1 ? 1 : dt == 2 ? 2 : 3;
+    D8WideArgs a{(const uint16_t*)dy, (const int8_t*)codes, (const uint8_t*)scales, (float*)dw,
+                 (float*)db, slab, slab + p.slab, dys, p.rps, (int)M, (int)(terms * M), N, K, kb,
+                 p.ntiles, p.ktiles,
+                 p.splits, add};
+    if (p.terms) {
+      uint16_t* t = (uint16_t*)(slab + p.slab + p.parts);
+      const long long blocks = (M * (p.N8 >> 3) + kNT - 1) / kNT;
+      const dim3 g((unsigned)(blocks < (1 << 16) ? blocks : (1 << 16)));
+      if (dt == 0)
+        hipLaunchKernelGGL(dense8_terms_kernel<0>, g, dim3(kNT), 0, st, dy, dys, M, N, p.N8, t);
+      if (dt == 1)
+        hipLaunchKernelGGL(dense8_terms_kernel<1>, g, dim3(kNT), 0, st, dy, dys, M, N, p.N8, t);
+      if (dt == 2)
+        hipLaunchKernelGGL(dense8_terms_kernel<2>, g, dim3(kNT), 0, st, dy, dys, M, N, p.N8, t);
+      ZK_CHECK_LAUNCH();
+      a.dy = t;
+      a.dys = p.N8;
+    }
+    const int e = dense8_wide_launch(a, st);
+    if (e) return e;
+  } else {
+    D8Args a{dy, (const int8_t*)codes, (const uint8_t*)scales, (float*)dw, (float*)db, slab,
+             slab + p.slab, dys, M, N, K, kb, p.ntiles, p.ktiles, p.splits, add, p.rps};
+    const dim3 g((unsigned)((long long)p.ntiles * p.ktiles * p.splits));
+    if (dt == 0) hipLaunchKernelGGL(dense8_wgrad_kernel<0>, g, dim3(kNT), 0, st, a);
+    if (dt == 1) hipLaunchKernelGGL(dense8_wgrad_kernel<1>, g, dim3(kNT), 0, st, a);
+    if (dt == 2) hipLaunchKernelGGL(dense8_wgrad_kernel<2>, g, dim3(kNT), 0, st, a);
+    ZK_CHECK_LAUNCH();
+  }
   const long long n = (long long)N * K;
   if (p.splits > 1)
     hipLaunchKernelGGL(dense8_sum_kernel, dim3((unsigned)((n + 63) / 64)), dim3(1024), 0, st,
-                       (const float*)ws, p.splits, n, (float*)dw, add & 1);
+                       (const float*)slab, p.splits, n, (float*)dw, add & 1);
   if (db)
     hipLaunchKernelGGL(dense8_sum_kernel, dim3((unsigned)((N + 63) / 64)), dim3(1024), 0, st,
-                       (const float*)ws + p.slab, p.splits * p.ktiles, (long long)N, (float*)db,
+                       (const float*)slab + p.slab, p.splits * p.ktiles, (long long)N, (float*)db,
                        (add >> 1) & 1);
   ZK_CHECK_LAUNCH();
   return 0;

@@ -121,8 +121,8 @@ SIGNATURES = {
     "zk_unpack8": (I32, [P] * 3 + [I64] * 2 + [I32, P]),
     "zk_gelu8_fwd": (I32, [P] * 4 + [I64] * 3 + [I32, P]),
     "zk_gelu8_bwd": (I32, [P] * 4 + [I64] * 3 + [I32, P]),
-    "zk_dense8_wgrad_ws_bytes": (I64, [I64, I32, I32]),
-    "zk_dense8_wgrad": (I32, [P] * 6 + [I64, I64, I32, I32, I64, I32, I32, P]),
+    "zk_dense8_wgrad_ws_bytes": (I64, [I64, I32, I32, I64, I32, I32, I32]),
+    "zk_dense8_wgrad": (I32, [P] * 6 + [I64, I64, I32, I32, I64, I32, I32, I32, P]),
     # classifier head: (ReLU) + global average pool + fp32 dense layer
     "zk_head_fwd": (I32, [P, P, P, P, P] + [I32] * 5 + [P]),
     "zk_head_bwd": (I32, [P] * 8 + [I32] * 5 + [P]),

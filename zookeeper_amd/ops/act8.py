@@ -205,29 +205,34 @@ def gelu8(x: torch.Tensor) -> torch.Tensor:
 
 # --- dense ------------------------------------------------------------------------
 
-def _dense_grads(dy, codes, scales, want_w: bool, want_b: bool, dw=None, db=None):
+def _dense_grads(dy, codes, scales, want_b: bool, dw=None, db=None, variant: int = -1):
     """fp32 ``dw`` [N, K] and ``db`` [N] of ``dy`` [..., N] and the kept input
-    [..., K]; given ``dw`` / ``db`` buffers are added to."""
+    [..., K]; given ``dw`` / ``db`` buffers are added to.  ``variant`` picks a
+    kernel (-1: by size)."""
     N, K = dy.shape[-1], codes.shape[-1]
     dev = dy.device
     dy2, rows, stride = rows_of(dy)
+    if stride >= 1 << 24:  # the kernels' row offsets are 32-bit
+        dy2, stride = dy2.contiguous(), N
     add = (1 if dw is not None else 0) | (2 if db is not None else 0)
     new = torch.zeros if rows == 0 else torch.empty
-    if want_w and dw is None:
+    if dw is None:
         dw = new((N, K), dtype=torch.float32, device=dev)
     if want_b and db is None:
         db = new((N,), dtype=torch.float32, device=dev)
     if rows == 0:
         return dw, db
     L = lib()
-    ws_bytes = L.zk_dense8_wgrad_ws_bytes(rows, N, K)
+    dt = DTYPE_CODES[dy.dtype]
+    ws_bytes = L.zk_dense8_wgrad_ws_bytes(rows, N, K, stride, dt, dy2.data_ptr() % 16 == 0,
+                                          variant)
     if ws_bytes < 0:
         raise ValueError(f"dense8: sizes rows={rows}, outputs={N}, inputs={K} are not supported")
     ws = torch.empty(max(ws_bytes // 4, 1), dtype=torch.float32, device=dev)
     with guard(dy):
         check(L.zk_dense8_wgrad(dy2.data_ptr(), codes.data_ptr(), scales.data_ptr(),
                                 dw.data_ptr(), ptr(db) if want_b else None, ws.data_ptr(),
-                                ws_bytes, rows, N, K, stride, DTYPE_CODES[dy.dtype], add,
+                                ws_bytes, rows, N, K, stride, dt, add, variant,
                                 stream_ptr(dev)), "zk_dense8_wgrad")
     return dw, db
 
@@ -249,7 +254,7 @@ def dense8_grads(dy: torch.Tensor, kept: Packed8,
         raise ValueError(f"dense8_grads: dy on {dy.device}, the kept input on {kept.device}")
     dy = dy.detach()
     if use_kernels(dy, "dense8_grads"):
-        return _dense_grads(dy, kept.codes, kept.scales, True, bias)
+        return _dense_grads(dy, kept.codes, kept.scales, bias)
     d = dy.reshape(-1, dy.shape[-1]).float()
     x = _unpack_plain(kept.codes, kept.scales, torch.float32).reshape(-1, kept.shape[-1])
     return d.t() @ x, d.sum(0) if bias else None
@@ -280,7 +285,7 @@ class _Dense8Fn(torch.autograd.Function):
         dw_direct = direct_grad(wp) if need_w and native else None
         db_direct = direct_grad(bp) if need_b and native else None
         if need_w and native:
-            dw, db = _dense_grads(dy, codes, scales, True, need_b, dw_direct, db_direct)
+            dw, db = _dense_grads(dy, codes, scales, need_b, dw_direct, db_direct)
         elif need_w:
             dw, db = dense8_grads(dy, Packed8(codes, scales, dy.dtype), need_b)
         elif need_b:  # a frozen weight with a trainable bias
