@@ -339,10 +339,10 @@ __global__ __launch_bounds__(kNT, 2) void dense8_wgrad_kernel(D8Args a) {
       const int o = r * 256 + (((tid & 15) ^ tr_swz<256>(r)) << 4);
       if constexpr (TERMS == 1) {
         uint4 w;
-        w.x = zk::pack_bf16x2(dreg[i][0], dreg[i][1]);
-        w.y = zk::pack_bf16x2(dreg[i][2], dreg[i][3]);
-        w.z = zk::pack_bf16x2(dreg[i][4], dreg[i][5]);
-        w.w = zk::pack_bf16x2(dreg[i][6], dreg[i][7]);
+        w.x = bf16_pair(dreg[i][0], dreg[i][1]);
+        w.y = bf16_pair(dreg[i][2], dreg[i][3]);
+        w.z = bf16_pair(dreg[i][4], dreg[i][5]);
+        w.w = bf16_pair(dreg[i][6], dreg[i][7]);
         *reinterpret_cast<uint4*>(buf + o) = w;
       } else {
 #pragma unroll
@@ -364,7 +364,7 @@ __global__ __launch_bounds__(kNT, 2) void dense8_wgrad_kernel(D8Args a) {
 #pragma unroll
       for (int j = 0; j < 4; ++j) {
         const uint32_t c = creg[2 * h + (j >> 1)];
-        w[j] = zk::pack_bf16x2(code_at(c, 2 * (j & 1)) * step, code_at(c, 2 * (j & 1) + 1) * step);
+        w[j] = bf16_pair(code_at(c, 2 * (j & 1)) * step, code_at(c, 2 * (j & 1) + 1) * step);
       }
       *reinterpret_cast<uint4*>(xb + xr * 256 +
                                 ((((tid & 7) * 2 + h) ^ tr_swz<256>(xr)) << 4)) =
@@ -453,10 +453,15 @@ __global__ __launch_bounds__(kNT, 2) void dense8_wgrad_kernel(D8Args a) {
 // per dy piece, 4 per code piece).  Behind the last row both kinds read valid
 // stand-ins, so the counts never change.
 //
+// The rows of a term are padded to whole steps (Mp = M rounded up to 64): dy rows
+// behind M are zeros, so the kept rows beside them may be any that exist.  (A NaN
+// block among those makes its columns of dW NaN, which they are anyway: the row is
+// part of the sum.)
+//
 // dy needs whole 16-byte chunks (N and the row stride multiples of 8, 16-byte
 // base).  Any other dy, and fp16 / fp32, is first cut into its bf16 terms,
-// [term][M][N8], and the product runs over the terms' rows one after the other
-// (virtual row r: kept row r mod M).
+// [term][Mp][N8], and the product runs over the terms one after the other (virtual
+// row r: kept row r mod Mp).
 // ---------------------------------------------------------------------------
 constexpr int kW = 256;                 // tile edge
 constexpr int kWNT = 512;               // threads
@@ -466,19 +471,26 @@ constexpr int kWBuf = 4 * kWPiece;      // dy halves 0 and 1, x halves 0 and 1
 __device__ __attribute__((aligned(512))) uint4 g_a8_zero[32];  // 512 B of zeros
 
 struct D8WideArgs {
-  const uint16_t* dy;     // [R][dys] bf16, R = terms * M
+  const uint16_t* dy;     // [dyrows][dys] bf16
   const int8_t* codes;    // [M][K]
   const uint8_t* scales;  // [M][kb]
   float* dw;
   float* db;
   float* slab;
   float* part;
-  long long dys, rps;  // rps: virtual rows of a split (multiple of 64)
-  int M, R, N, K, kb, ntiles, ktiles, splits, add;
+  long long dys;
+  int rps;                // virtual rows of a split (multiple of 64)
+  int dyrows;             // rows that exist: M, or all R of the terms
+  int M, Mp, R, N, K, kb, ntiles, ktiles, splits, add;
 };
 
-// 16 bytes per lane to LDS address lds (wave-uniform) + 16 * lane
-__device__ __forceinline__ void dma16(const void* src, uint32_t lds) {
+// 16 bytes per lane to LDS address lds (wave-uniform) + 16 * lane, from a uniform
+// base and 32-bit lane offsets, or from an address per lane
+__device__ __forceinline__ void dma16(const void* base, uint32_t off, uint32_t lds) {
+  asm volatile("s_mov_b32 m0, %2\n\tglobal_load_lds_dwordx4 %0, %1" ::"v"(off), "s"(base), "s"(lds)
+               : "m0", "memory");
+}
+__device__ __forceinline__ void dma16_any(const void* src, uint32_t lds) {
   asm volatile("s_mov_b32 m0, %1\n\tglobal_load_lds_dwordx4 %0, off" ::"v"(src), "s"(lds)
                : "m0", "memory");
 }
@@ -487,13 +499,12 @@ __device__ __forceinline__ void lds_barrier() {
   asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory");
 }
 
+// KCUT: K is no multiple of 8.  All LDS is dynamic and addressed by byte from 0.
+template <bool KCUT>
 __global__ __launch_bounds__(kWNT, 2) void dense8_wide_kernel(D8WideArgs a) {
-  extern __shared__ __attribute__((aligned(1024))) unsigned char smem[];
-  typedef __attribute__((address_space(3))) unsigned char lds_u8;
   typedef __attribute__((address_space(3))) s16x4 lds_s16x4;
   typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
   typedef __attribute__((address_space(3))) u32x4 lds_u128;
-  const uint32_t lds0 = (uint32_t)(uintptr_t)(lds_u8*)smem;
   const int tid = threadIdx.x, lane = tid & 63;
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int wn = wave >> 2, wk = wave & 3;
@@ -503,8 +514,8 @@ __global__ __launch_bounds__(kWNT, 2) void dense8_wide_kernel(D8WideArgs a) {
   const int kt = tile % a.ktiles, nt = tile / a.ktiles;
   const int n0 = nt * kW, k0 = kt * kW;
   // R < 2^31 - 256: the steps that run ahead of the last row fit too
-  const int r0 = (int)(split * a.rps), r1 = (int)min((long long)a.R, r0 + a.rps);
-  const int steps = (r1 - r0 + 63) >> 6;
+  const int r0 = split * a.rps, r1 = min(a.R, r0 + a.rps);
+  const int steps = (r1 - r0) >> 6;
 
   // dy: instruction i of wave w fills piece rows (8 i + w) * 2 + (lane >> 5); LDS slot
   // lane & 31 holds the row's 16-byte chunk (lane & 31) ^ tr_swz(row).  Chunks behind N
@@ -512,65 +523,82 @@ __global__ __launch_bounds__(kWNT, 2) void dense8_wide_kernel(D8WideArgs a) {
   const int arow = wave * 2 + (lane >> 5);  // i = 1: + 16, the same swizzle
   const int chunk = (lane & 31) ^ tr_swz<512>(arow);
   const int acol = n0 + chunk * 8 < a.N ? chunk * 16 : 0;
-  const unsigned char* dyb = reinterpret_cast<const unsigned char*>(a.dy) + n0 * 2LL + acol;
-  const unsigned char* zero = reinterpret_cast<const unsigned char*>(g_a8_zero) + chunk * 16;
-  const uint32_t dyrow = (uint32_t)a.dys * 2u;
+  const unsigned char* dyb = reinterpret_cast<const unsigned char*>(a.dy) + n0 * 2LL;
+  const long long dyrow = a.dys * 2;
+  const uint32_t aoff = (uint32_t)(arow * (int)dyrow + acol);
   auto issue = [&](int s, int h) {
-    const uint32_t dst = lds0 + (s & 1) * kWBuf + h * kWPiece + wave * 1024;
-    const int rb = r0 + s * 64 + h * 32 + arow;
+    const uint32_t dst = (s & 1) * kWBuf + h * kWPiece + wave * 1024;
+    const int rb = r0 + s * 64 + h * 32;  // uniform
+    if (rb + 32 <= a.dyrows) {
+      const unsigned char* base = dyb + rb * dyrow;
+      dma16(base, aoff, dst);
+      dma16(base + 16 * dyrow, aoff, dst + 8192);
+    } else {
 #pragma unroll
-    for (int i = 0; i < 2; ++i) {
-      const int r = rb + 16 * i;
-      dma16(r < r1 ? dyb + (u64_t)(uint32_t)r * dyrow : zero, dst + i * 8192);
+      for (int i = 0; i < 2; ++i) {
+        const int r = rb + arow + 16 * i;
+        const unsigned char* src = reinterpret_cast<const unsigned char*>(g_a8_zero) + chunk * 16;
+        if (r < a.dyrows) src = dyb + r * dyrow + acol;
+        dma16_any(src, dst + i * 8192);
+      }
     }
   };
 
   // codes: 8 of columns 8 (tid & 31) of rows tid >> 5 and + 16 of a half.  A chunk that K
   // cuts is read from the row's last 8 and moved down; columns behind K: any valid place.
-  // Rows behind the split: the first one (put() makes them zeros).
   const int crow = tid >> 5, col = k0 + (tid & 31) * 8;
-  const int cc = col >= a.K ? 0 : min(col, a.K - 8);
+  const int cc = col >= a.K ? 0 : KCUT ? min(col, a.K - 8) : col;
   const int back = col >= a.K ? 0 : 8 * (col - cc);
-  const int8_t* cp = a.codes + cc;
-  const uint8_t* sp = a.scales + ((col >= a.K ? 0 : col) >> 5);
+  const int sc = (col >= a.K ? 0 : col) >> 5;
   struct Codes {
     Bytes8 w[2];
     uint32_t e[2];
   };
   auto fetch = [&](Codes& c, int s, int h) {
-    const int rb = r0 + s * 64 + h * 32;  // uniform
-    int mb = rb >= a.M ? rb - a.M : rb;   // row in its term: at most two terms back
-    mb = mb >= a.M ? mb - a.M : mb;
+    int mb = r0 + s * 64 + h * 32;  // uniform; row in its term
 #pragma unroll
-    for (int i = 0; i < 2; ++i) {
-      int m = mb + crow + 16 * i;
-      m = m >= a.M ? m - a.M : m;  // the next term starts inside the piece (M >= 64)
-      m = rb + crow + 16 * i < r1 ? m : 0;
-      c.w[i] = *reinterpret_cast<const Bytes8*>(cp + (u64_t)(uint32_t)m * (uint32_t)a.K);
-      c.e[i] = sp[(u64_t)(uint32_t)m * (uint32_t)a.kb];
+    for (int i = 0; i < 3; ++i) mb = mb >= a.Mp ? mb - a.Mp : mb;  // past the last: any row
+    mb = mb >= a.Mp ? 0 : mb;
+    const int m0 = min(mb, a.M - 1);
+    int ra = crow, rb = crow + 16;
+    if (mb + 32 > a.M) {  // rows behind M: the last one
+      ra = min(ra, a.M - 1 - m0);
+      rb = min(rb, a.M - 1 - m0);
     }
+    const int8_t* p = a.codes + (long long)m0 * a.K;
+    const uint8_t* q = a.scales + (long long)m0 * a.kb;
+    c.w[0] = *reinterpret_cast<const Bytes8*>(p + (uint32_t)(ra * a.K + cc));
+    c.e[0] = q[(uint32_t)(ra * a.kb + sc)];
+    c.w[1] = *reinterpret_cast<const Bytes8*>(p + (uint32_t)(rb * a.K + cc));
+    c.e[1] = q[(uint32_t)(rb * a.kb + sc)];
   };
   // the other 16 rows of a half have the same swizzle
-  uint32_t xput = crow * 512 + (((tid & 31) ^ tr_swz<512>(crow)) << 4);
+  const uint32_t xput = crow * 512 + (((tid & 31) ^ tr_swz<512>(crow)) << 4);
   auto put = [&](const Codes& c, int s, int h) {
-    const uint32_t at = lds0 + (xput ^ ((s & 1) * kWBuf));
+    const uint32_t at = xput | ((s & 1) * kWBuf);
 #pragma unroll
     for (int i = 0; i < 2; ++i) {
-      const bool live = r0 + s * 64 + h * 32 + 16 * i + crow < r1;
-      const float st = live ? step_of(c.e[i]) : 0.f;
+      // E = 255: the step is infinite and 0 codes become inf - inf = NaN
+      const uint32_t e = c.e[i];
+      const float st = __uint_as_float((e == 255u ? 255u : e - 6u) << 23);
       const float off = -128.f * st;
-      const u64_t v = (((u64_t)c.w[i][1] << 32) | c.w[i][0]) >> back;
-      const uint32_t b[2] = {(uint32_t)v ^ 0x80808080u, (uint32_t)(v >> 32) ^ 0x80808080u};
-      uint32_t o[4];
+      uint32_t b0 = c.w[i][0], b1 = c.w[i][1];
+      if constexpr (KCUT) {
+        const u64_t v = (((u64_t)b1 << 32) | b0) >> back;
+        b0 = (uint32_t)v;
+        b1 = (uint32_t)(v >> 32);
+      }
+      // code + 128 as an unsigned byte: the conversion picks the byte itself
+      const uint32_t b[2] = {b0 ^ 0x80808080u, b1 ^ 0x80808080u};
+      u32x4 o;
 #pragma unroll
       for (int j = 0; j < 4; ++j) {
-        // code + 128 as an unsigned byte: the conversion picks the byte itself
         const uint32_t w = b[j >> 1];
         const float x = (float)((w >> (16 * (j & 1))) & 0xffu);
         const float y = (float)((w >> (16 * (j & 1) + 8)) & 0xffu);
-        o[j] = zk::pack_bf16x2(__builtin_fmaf(x, st, off), __builtin_fmaf(y, st, off));
+        o[j] = bf16_pair(__builtin_fmaf(x, st, off), __builtin_fmaf(y, st, off));
       }
-      *(lds_u128*)(uintptr_t)(at + (2 + h) * kWPiece + i * 8192) = u32x4{o[0], o[1], o[2], o[3]};
+      *(lds_u128*)(uintptr_t)(at + (2 + h) * kWPiece + i * 8192) = o;
     }
   };
 
@@ -588,23 +616,23 @@ __global__ __launch_bounds__(kWNT, 2) void dense8_wide_kernel(D8WideArgs a) {
   // addresses would spill.
   const int q4 = (lane & 15) >> 2, p4 = lane & 3, frow = 8 * (lane >> 4) + q4;
   const uint32_t f0 = frow * 512 + (((p4 >> 1) ^ tr_swz<512>(frow)) << 4) + (p4 & 1) * 8;
-  uint32_t fd = f0 ^ (wn * 256), fx = f0 ^ (wk * 128);
+  const uint32_t fd = f0 ^ (wn * 256), fx = f0 ^ (wk * 128);
   auto frag = [&](uint32_t l, uint32_t block, uint32_t piece) {
-    const uint32_t at = lds0 + piece + (l ^ block);
-    const uint32_t at4 = lds0 + piece + 2048 + (l ^ block ^ 16u);
-    const s16x4 lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4*)(uintptr_t)at);
-    const s16x4 hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4*)(uintptr_t)at4);
+    const s16x4 lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16(
+        (lds_s16x4*)(uintptr_t)((l ^ block) + piece));
+    const s16x4 hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16(
+        (lds_s16x4*)(uintptr_t)((l ^ (block | 16u)) + (piece + 2048)));
     const s16x8 v = {lo[0], lo[1], lo[2], lo[3], hi[0], hi[1], hi[2], hi[3]};
     return __builtin_bit_cast(uint4, v);
   };
   auto readD = [&](uint4 (&d)[4], int s, int h, int mh) {
-    uint32_t l = fd ^ ((s & 1) * kWBuf);
+    uint32_t l = fd | ((s & 1) * kWBuf);
     asm volatile("" : "+v"(l));
 #pragma unroll
     for (int i = 0; i < 4; ++i) d[i] = frag(l, mh * 128 + i * 32, h * kWPiece);
   };
   auto readX = [&](uint4 (&d)[4], int s, int h) {
-    uint32_t l = fx ^ ((s & 1) * kWBuf);
+    uint32_t l = fx | ((s & 1) * kWBuf);
     asm volatile("" : "+v"(l));
 #pragma unroll
     for (int j = 0; j < 4; ++j) d[j] = frag(l, j * 32, (2 + h) * kWPiece);
@@ -647,11 +675,6 @@ __global__ __launch_bounds__(kWNT, 2) void dense8_wide_kernel(D8WideArgs a) {
     __builtin_amdgcn_sched_barrier(0);
     put(c0, s + 1, 0);
     mma(d1, x1, 0);
-#pragma unroll
-    for (int i = 0; i < 16; ++i) {
-      __builtin_amdgcn_sched_group_barrier(0x008, 1, 0);
-      __builtin_amdgcn_sched_group_barrier(0x002, 5, 0);
-    }
     __builtin_amdgcn_sched_barrier(0);
     if (sum) sums(d1, 0);
     issue(s + 1, 0);
@@ -670,11 +693,6 @@ __global__ __launch_bounds__(kWNT, 2) void dense8_wide_kernel(D8WideArgs a) {
     __builtin_amdgcn_sched_barrier(0);
     put(c1, s + 1, 1);
     mma(d1, x2, 0);
-#pragma unroll
-    for (int i = 0; i < 16; ++i) {
-      __builtin_amdgcn_sched_group_barrier(0x008, 1, 0);
-      __builtin_amdgcn_sched_group_barrier(0x002, 5, 0);
-    }
     __builtin_amdgcn_sched_barrier(0);
     if (sum) sums(d1, 0);
     issue(s + 1, 1);
@@ -721,33 +739,53 @@ __global__ __launch_bounds__(kWNT, 2) void dense8_wide_kernel(D8WideArgs a) {
   }
 }
 
-// dy [M][dys] -> its bf16 terms [TERMS][M][N8], columns behind N zero
+// dy [M][dys] -> its bf16 terms [TERMS][Mp][N8]; columns behind N and rows behind M zero
 template <int DT>
 __global__ __launch_bounds__(kNT) void dense8_terms_kernel(const void* dy, long long dys,
-                                                           long long M, int N, int N8,
-                                                           uint16_t* out) {
+                                                           long long M, long long Mp, int N,
+                                                           int N8, uint16_t* out) {
   constexpr int TERMS = DT == 1 ? 1 : DT == 2 ? 2 : 3;
   typedef typename Elem<DT>::raw raw;
   const int chunks = N8 >> 3;
-  const long long total = M * chunks, step = (long long)gridDim.x * kNT;
+  const long long total = Mp * chunks, step = (long long)gridDim.x * kNT;
   for (long long id = (long long)blockIdx.x * kNT + threadIdx.x; id < total; id += step) {
-    const long long m = id / chunks;
+    const long long m = total < (1LL << 31) ? (uint32_t)id / (uint32_t)chunks : id / chunks;
     const int c = (int)(id - m * chunks) * 8;
     float f[8];
-    load8_n<DT>(reinterpret_cast<const raw*>(dy) + m * dys + c, N - c, 0.f, f);
+    load8_n<DT>(reinterpret_cast<const raw*>(dy) + m * dys + c, m < M ? N - c : 0, 0.f, f);
 #pragma unroll
     for (int t = 0; t < TERMS; ++t) {
       uint32_t h[8];
 #pragma unroll
       for (int j = 0; j < 8; ++j) h[j] = cut_term(f[j]);
-      *reinterpret_cast<uint4*>(out + ((long long)t * M + m) * N8 + c) =
+      *reinterpret_cast<uint4*>(out + (t * Mp + m) * N8 + c) =
           uint4{h[0] | (h[1] << 16), h[2] | (h[3] << 16), h[4] | (h[5] << 16), h[6] | (h[7] << 16)};
     }
   }
 }
 
-// out[i] (+)= sum over p of part[p][i]: 16 slices of the parts side by side, each in
-// order, joined in order
+// out[i] (+)= sum over p of part[p][i].  Few parts: 4 values per thread, the parts in
+// order.
+__global__ __launch_bounds__(kNT) void dense8_sum4_kernel(const float* __restrict__ part,
+                                                          int parts, long long n,
+                                                          float* __restrict__ out, int add) {
+  const long long i = ((long long)blockIdx.x * kNT + threadIdx.x) * 4;
+  if (i >= n) return;
+  if (i + 4 <= n && (n & 3) == 0) {
+    f32x4 s = *reinterpret_cast<const f32x4*>(part + i);
+    for (int p = 1; p < parts; ++p) s += *reinterpret_cast<const f32x4*>(part + p * n + i);
+    if (add) s += *reinterpret_cast<const f32x4*>(out + i);
+    *reinterpret_cast<f32x4*>(out + i) = s;
+  } else {
+    for (long long j = i; j < n && j < i + 4; ++j) {
+      float s = part[j];
+      for (int p = 1; p < parts; ++p) s += part[p * n + j];
+      out[j] = add ? s + out[j] : s;
+    }
+  }
+}
+
+// Many parts: 16 slices of them side by side, each in order, joined in order.
 __global__ __launch_bounds__(1024) void dense8_sum_kernel(const float* __restrict__ part,
                                                           int parts, long long n,
                                                           float* __restrict__ out, int add) {
@@ -764,6 +802,16 @@ __global__ __launch_bounds__(1024) void dense8_sum_kernel(const float* __restric
     for (int o = 1; o < 16; ++o) s += red[o][col];
     out[i] = add ? out[i] + s : s;
   }
+}
+
+int dense8_sum(const float* part, int parts, long long n, float* out, int add, hipStream_t st) {
+  if (parts <= 8 || n >= (1 << 20))
+    hipLaunchKernelGGL(dense8_sum4_kernel, dim3((unsigned)((n + 4 * kNT - 1) / (4 * kNT))),
+                       dim3(kNT), 0, st, part, parts, n, out, add);
+  else
+    hipLaunchKernelGGL(dense8_sum_kernel, dim3((unsigned)((n + 63) / 64)), dim3(1024), 0, st, part,
+                       parts, n, out, add);
+  return (int)hipGetLastError();
 }
 
 // Sizes and workspace of one call.  wide: the 256 x 256 kernel.
@@ -792,7 +840,7 @@ D8Plan dense8_plan(long long M, int N, int K, int dt, long long dys, bool aligne
   if (p.wide) {
     // one block per CU and about a microsecond per step: the split that takes the fewest
     // rounds of steps (12 more per block for its start and end) and slab bytes
-    const long long R = terms * M;
+    const long long R = terms * ((M + 63) / 64 * 64);
     double best = 1e30;
     for (long long c = 1; c <= 64 && (c == 1 || R / c >= 512); ++c) {
       const double rounds = (double)((tiles * c + 255) / 256);
@@ -818,7 +866,7 @@ D8Plan dense8_plan(long long M, int N, int K, int dt, long long dys, bool aligne
   p.parts = (long long)p.splits * p.ktiles * N;
   p.slab = (p.slab + 3) & ~3LL;
   p.parts = (p.parts + 3) & ~3LL;  // the terms start 16-byte aligned
-  p.bytes = 4 * (p.slab + p.parts) + (p.terms ? 2LL * terms * M * p.N8 : 0);
+  p.bytes = 4 * (p.slab + p.parts) + (p.terms ? 2LL * terms * ((M + 63) / 64 * 64) * p.N8 : 0);
   return p;
 }
 
@@ -832,13 +880,18 @@ bool g_wide_attr = false;
 
 int dense8_wide_launch(const D8WideArgs& a, hipStream_t st) {
   if (!g_wide_attr) {
-    const hipError_t e = hipFuncSetAttribute((const void*)dense8_wide_kernel,
-                                             hipFuncAttributeMaxDynamicSharedMemorySize, 2 * kWBuf);
-    if (e != hipSuccess) return (int)e;
+    for (const void* f : {(const void*)dense8_wide_kernel<false>, (const void*)dense8_wide_kernel<true>}) {
+      const hipError_t e =
+          hipFuncSetAttribute(f, hipFuncAttributeMaxDynamicSharedMemorySize, 2 * kWBuf);
+      if (e != hipSuccess) return (int)e;
+    }
     g_wide_attr = true;
   }
-  hipLaunchKernelGGL(dense8_wide_kernel, dim3((unsigned)(a.ntiles * a.ktiles * a.splits)),
-                     dim3(kWNT), 2 * kWBuf, st, a);
+  const dim3 g((unsigned)(a.ntiles * a.ktiles * a.splits));
+  if (a.K & 7)
+    hipLaunchKernelGGL(dense8_wide_kernel<true>, g, dim3(kWNT), 2 * kWBuf, st, a);
+  else
+    hipLaunchKernelGGL(dense8_wide_kernel<false>, g, dim3(kWNT), 2 * kWBuf, st, a);
   return (int)hipGetLastError();
 }
 
@@ -896,23 +949,24 @@ ZK_EXPORT int zk_dense8_wgrad(const void* dy, const void* codes, const void* sca
   float* const slab = (float*)ws;
   if (p.wide) {
     const int terms = dt == 1 ? 1 : dt == 2 ? 2 : 3;
+    const int Mp = (int)((M + 63) / 64 * 64);
     D8WideArgs a{(const uint16_t*)dy, (const int8_t*)codes, (const uint8_t*)scales, (float*)dw,
-                 (float*)db, slab, slab + p.slab, dys, p.rps, (int)M, (int)(terms * M), N, K, kb,
-                 p.ntiles, p.ktiles,
-                 p.splits, add};
+                 (float*)db, slab, slab + p.slab, dys, (int)p.rps, (int)M, (int)M, Mp,
+                 terms * Mp, N, K, kb, p.ntiles, p.ktiles, p.splits, add};
     if (p.terms) {
       uint16_t* t = (uint16_t*)(slab + p.slab + p.parts);
-      const long long blocks = (M * (p.N8 >> 3) + kNT - 1) / kNT;
+      const long long blocks = ((long long)Mp * (p.N8 >> 3) + kNT - 1) / kNT;
       const dim3 g((unsigned)(blocks < (1 << 16) ? blocks : (1 << 16)));
       if (dt == 0)
-        hipLaunchKernelGGL(dense8_terms_kernel<0>, g, dim3(kNT), 0, st, dy, dys, M, N, p.N8, t);
+        hipLaunchKernelGGL(dense8_terms_kernel<0>, g, dim3(kNT), 0, st, dy, dys, M, Mp, N, p.N8, t);
       if (dt == 1)
-        hipLaunchKernelGGL(dense8_terms_kernel<1>, g, dim3(kNT), 0, st, dy, dys, M, N, p.N8, t);
+        hipLaunchKernelGGL(dense8_terms_kernel<1>, g, dim3(kNT), 0, st, dy, dys, M, Mp, N, p.N8, t);
       if (dt == 2)
-        hipLaunchKernelGGL(dense8_terms_kernel<2>, g, dim3(kNT), 0, st, dy, dys, M, N, p.N8, t);
+        hipLaunchKernelGGL(dense8_terms_kernel<2>, g, dim3(kNT), 0, st, dy, dys, M, Mp, N, p.N8, t);
       ZK_CHECK_LAUNCH();
       a.dy = t;
       a.dys = p.N8;
+      a.dyrows = a.R;
     }
     const int e = dense8_wide_launch(a, st);
     if (e) return e;
@@ -925,14 +979,9 @@ ZK_EXPORT int zk_dense8_wgrad(const void* dy, const void* codes, const void* sca
     if (dt == 2) hipLaunchKernelGGL(dense8_wgrad_kernel<2>, g, dim3(kNT), 0, st, a);
     ZK_CHECK_LAUNCH();
   }
-  const long long n = (long long)N * K;
-  if (p.splits > 1)
-    hipLaunchKernelGGL(dense8_sum_kernel, dim3((unsigned)((n + 63) / 64)), dim3(1024), 0, st,
-                       (const float*)slab, p.splits, n, (float*)dw, add & 1);
-  if (db)
-    hipLaunchKernelGGL(dense8_sum_kernel, dim3((unsigned)((N + 63) / 64)), dim3(1024), 0, st,
-                       (const float*)slab + p.slab, p.splits * p.ktiles, (long long)N, (float*)db,
-                       (add >> 1) & 1);
-  ZK_CHECK_LAUNCH();
-  return 0;
+  if (p.splits > 1) {
+    const int e = dense8_sum(slab, p.splits, (long long)N * K, (float*)dw, add & 1, st);
+    if (e) return e;
+  }
+  return db ? dense8_sum(slab + p.slab, p.splits * p.ktiles, N, (float*)db, (add >> 1) & 1, st) : 0;
 }

@@ -74,6 +74,23 @@ __device__ __forceinline__ void load8_n(const typename Elem<DT>::raw* p, int n, 
   }
 }
 
+// Two values to bf16 in one v_cvt_pk_bf16_f32 (two separate conversions take four
+// instructions).
+__device__ __forceinline__ uint32_t bf16_pair(float lo, float hi) {
+  typedef float f32x2 __attribute__((ext_vector_type(2)));
+  typedef __bf16 b16x2 __attribute__((ext_vector_type(2)));
+  return __builtin_bit_cast(uint32_t, __builtin_convertvector(f32x2{lo, hi}, b16x2));
+}
+
+template <int DT>
+__device__ __forceinline__ uint32_t pair16(float lo, float hi) {
+  if constexpr (DT == 1) {
+    return bf16_pair(lo, hi);
+  } else {
+    return (uint32_t)Elem<DT>::down(lo) | ((uint32_t)Elem<DT>::down(hi) << 16);
+  }
+}
+
 template <int DT>
 __device__ __forceinline__ void store8(typename Elem<DT>::raw* p, const float (&f)[8]) {
   if constexpr (DT == 0) {
@@ -88,8 +105,7 @@ __device__ __forceinline__ void store8(typename Elem<DT>::raw* p, const float (&
   } else {
     Bytes16 a;
 #pragma unroll
-    for (int i = 0; i < 4; ++i)
-      a[i] = (uint32_t)Elem<DT>::down(f[2 * i]) | ((uint32_t)Elem<DT>::down(f[2 * i + 1]) << 16);
+    for (int i = 0; i < 4; ++i) a[i] = pair16<DT>(f[2 * i], f[2 * i + 1]);
     *reinterpret_cast<Bytes16*>(p) = a;
   }
 }
