@@ -423,3 +423,23 @@ def test_the_operators_together():
     for got, want in pairs:
         # each value is a sum of at most 132 * 96 terms through five fp32 layers
         assert (got.double() - want).norm() <= 2e-5 * want.norm()
+
+
+def test_gradients_of_other_layouts():
+    """Incoming gradients that are transposed, sliced or broadcast."""
+    from zookeeper_amd.ops import dense8, gelu8
+
+    torch.manual_seed(6)
+    for shape in ((12, 40), (3, 4, 40)):
+        x = torch.randn(shape, device="cuda", requires_grad=True)
+        w = torch.randn(40, 40, device="cuda", requires_grad=True)
+        flip = torch.randn(*reversed(shape), device="cuda").permute(*reversed(range(len(shape))))
+        wide = torch.randn(*shape[:-1], 57, device="cuda")[..., 9:49]
+        row = torch.randn(40, device="cuda").expand(shape)
+        for dy in (flip, wide, row):
+            got, = torch.autograd.grad(gelu8(x), x, dy)
+            want, = torch.autograd.grad(gelu8(x), x, dy.contiguous())
+            assert torch.equal(got, want)
+            got, = torch.autograd.grad(dense8(x, w), w, dy)
+            want, = torch.autograd.grad(dense8(x, w), w, dy.contiguous())
+            assert torch.equal(got, want)

@@ -262,3 +262,21 @@ def test_second_derivative_is_refused():
     x = torch.randn(4, 32, device="cuda", requires_grad=True)
     with pytest.raises(RuntimeError, match="not differentiable"):
         torch.autograd.grad(layer_norm(x).sum(), x, create_graph=True)
+
+
+def test_gradients_of_other_layouts():
+    """Incoming gradients that are transposed, sliced or broadcast, two and three
+    dimensions: dx has the input's shape, row by row."""
+    from zookeeper_amd.ops import layer_norm
+
+    torch.manual_seed(6)
+    for shape in ((12, 40), (3, 4, 40)):
+        x = torch.randn(shape, device="cuda", requires_grad=True)
+        w = torch.rand(40, device="cuda", requires_grad=True)
+        flip = torch.randn(*reversed(shape), device="cuda").permute(*reversed(range(len(shape))))
+        wide = torch.randn(*shape[:-1], 57, device="cuda")[..., 9:49]
+        row = torch.randn(40, device="cuda").expand(shape)
+        for dy in (flip, wide, row):
+            got = torch.autograd.grad(layer_norm(x, w), [x, w], dy)
+            want = torch.autograd.grad(layer_norm(x, w), [x, w], dy.contiguous())
+            assert all(torch.equal(a, b) for a, b in zip(got, want))

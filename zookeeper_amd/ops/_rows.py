@@ -14,7 +14,17 @@ from zookeeper_amd.ops import _native
 # element type codes of the C ABI (csrc/kernels/rows.h)
 DTYPE_CODES = {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2}
 
+# Raw hipStream_t of torch's current stream on a device index.
+raw_stream = torch._C._cuda_getCurrentRawStream
+
 _HERE = contextlib.nullcontext()
+
+
+def call(fn, what: str, *args) -> None:
+    """A native launch and its error check."""
+    rc = fn(*args)
+    if rc or _native._DEBUG_SYNC:
+        _native.check(rc, what)
 
 
 def use_kernels(t: torch.Tensor, what: str) -> bool:
@@ -31,8 +41,9 @@ def use_kernels(t: torch.Tensor, what: str) -> bool:
 
 
 def guard(t: torch.Tensor):
-    """Context that makes ``t``'s device the current one for a launch."""
-    if t.device.index == torch.cuda.current_device():
+    """Context that makes ``t``'s device the current one for a launch.  (A backward
+    needs none: autograd runs it on a thread of its tensors' device.)"""
+    if t.device.index == torch._C._cuda_getDevice():
         return _HERE
     return torch.cuda.device(t.device)
 
@@ -71,9 +82,8 @@ def ptr(t):
     return None if t is None else t.data_ptr()
 
 
-def once_only(what: str) -> None:
-    """Called in a backward: the kernels' gradients are not differentiable
-    themselves, so refuse ``create_graph=True`` (the only way that gradients are
-    recorded here) instead of returning constants."""
-    if torch.is_grad_enabled():
-        raise RuntimeError(f"{what}: the gradient is not differentiable (create_graph=True)")
+def refuse_twice(what: str) -> None:
+    """Raised by a backward that runs with gradients recorded, which is what
+    ``create_graph=True`` does: the kernels' gradients are not differentiable
+    themselves and would count as constants."""
+    raise RuntimeError(f"{what}: the gradient is not differentiable (create_graph=True)")

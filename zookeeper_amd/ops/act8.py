@@ -29,8 +29,9 @@ from typing import Optional, Tuple
 import torch
 import torch.nn.functional as F
 
-from zookeeper_amd.ops._native import check, direct_grad, grad_ready, lib, stream_ptr
-from zookeeper_amd.ops._rows import DTYPE_CODES, guard, once_only, ptr, rows_of, use_kernels
+from zookeeper_amd.ops._native import direct_grad, grad_ready, lib
+from zookeeper_amd.ops._rows import (DTYPE_CODES, call, guard, ptr, raw_stream, refuse_twice,
+                                     rows_of, use_kernels)
 
 BLOCK = 32
 
@@ -129,9 +130,8 @@ def pack8(x: torch.Tensor) -> Packed8:
     codes, scales = _empty_form(x)
     x2, rows, stride = rows_of(x)
     with guard(x):
-        check(lib().zk_pack8(x2.data_ptr(), codes.data_ptr(), scales.data_ptr(), rows,
-                             x.shape[-1], stride, DTYPE_CODES[x.dtype], stream_ptr(x.device)),
-              "zk_pack8")
+        call(lib().zk_pack8, "zk_pack8", x2.data_ptr(), codes.data_ptr(), scales.data_ptr(), rows,
+             x.shape[-1], stride, DTYPE_CODES[x.dtype], raw_stream(x.device.index))
     return Packed8(codes, scales, x.dtype)
 
 
@@ -144,53 +144,69 @@ def unpack8(kept: Packed8, dtype: Optional[torch.dtype] = None) -> torch.Tensor:
         return _unpack_plain(kept.codes, kept.scales, dtype)
     n = kept.shape[-1]
     with guard(out):
-        check(lib().zk_unpack8(kept.codes.data_ptr(), kept.scales.data_ptr(), out.data_ptr(),
-                               out.numel() // n, n, DTYPE_CODES[dtype], stream_ptr(out.device)),
-              "zk_unpack8")
+        call(lib().zk_unpack8, "zk_unpack8", kept.codes.data_ptr(), kept.scales.data_ptr(),
+             out.data_ptr(), out.numel() // n, n, DTYPE_CODES[dtype],
+             raw_stream(out.device.index))
     return out
 
 
 # --- GELU -------------------------------------------------------------------------
 
 def _gelu_forward(x, keep: bool):
-    y = torch.empty(x.shape, dtype=x.dtype, device=x.device)
-    codes, scales = _empty_form(x) if keep else (None, None)
+    """``y`` and the kept input in one buffer: the codes, then the scales."""
     x2, rows, stride = rows_of(x)
+    n = x.shape[-1]
+    dev = x.device
+    y = torch.empty_like(x) if x.is_contiguous() else torch.empty(x.shape, dtype=x.dtype,
+                                                                  device=dev)
+    kept = codes = scales = None
+    if keep:
+        kept = torch.empty(rows * (n + (n + BLOCK - 1) // BLOCK), dtype=torch.uint8, device=dev)
+        codes = kept.data_ptr()
+        scales = codes + rows * n
     with guard(x):
-        check(lib().zk_gelu8_fwd(x2.data_ptr(), y.data_ptr(), ptr(codes), ptr(scales), rows,
-                                 x.shape[-1], stride, DTYPE_CODES[x.dtype],
-                                 stream_ptr(x.device)), "zk_gelu8_fwd")
-    return y, codes, scales
+        call(lib().zk_gelu8_fwd, "zk_gelu8_fwd", x2.data_ptr(), y.data_ptr(), codes, scales, rows,
+             n, stride, DTYPE_CODES[x.dtype], raw_stream(dev.index))
+    return y, kept, rows
 
 
 class _Gelu8Fn(torch.autograd.Function):
     @staticmethod
-    def forward(ctx, x, native):
-        if native:
-            y, codes, scales = _gelu_forward(x, True)
-        else:
-            y = F.gelu(x)
-            codes, scales = _pack_plain(x)
-        ctx.save_for_backward(codes, scales)
-        ctx.native = native
+    def forward(ctx, x):
+        y, kept, ctx.rows = _gelu_forward(x, True)
+        ctx.save_for_backward(kept)
         return y
 
     @staticmethod
     def backward(ctx, dy):
-        once_only("gelu8")
-        codes, scales = ctx.saved_tensors
-        if not ctx.native:
-            k = _unpack_plain(codes, scales, torch.float32).to(
-                torch.float64 if dy.dtype == torch.float64 else torch.float32)
-            return (dy.to(k.dtype) * _gelu_slope(k)).to(dy.dtype), None
-        dx = torch.empty(dy.shape, dtype=dy.dtype, device=dy.device)
-        dy2, rows, stride = rows_of(dy)
-        with guard(dy):
-            check(lib().zk_gelu8_bwd(dy2.data_ptr(), codes.data_ptr(), scales.data_ptr(),
-                                     dx.data_ptr(), rows, dy.shape[-1], stride,
-                                     DTYPE_CODES[dy.dtype], stream_ptr(dy.device)),
-                  "zk_gelu8_bwd")
-        return dx, None
+        if torch.is_grad_enabled():
+            refuse_twice("gelu8")
+        kept, = ctx.saved_tensors
+        n, rows, dev = dy.shape[-1], ctx.rows, dy.device
+        if dy.is_contiguous():
+            dx, dy2, stride = torch.empty_like(dy), dy, n
+        else:
+            dx = torch.empty(dy.shape, dtype=dy.dtype, device=dev)
+            dy2, _, stride = rows_of(dy)
+        codes = kept.data_ptr()
+        call(lib().zk_gelu8_bwd, "zk_gelu8_bwd", dy2.data_ptr(), codes, codes + rows * n,
+             dx.data_ptr(), rows, n, stride, DTYPE_CODES[dy.dtype], raw_stream(dev.index))
+        return dx
+
+
+class _Gelu8HostFn(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, x):
+        ctx.save_for_backward(*_pack_plain(x))
+        return F.gelu(x)
+
+    @staticmethod
+    def backward(ctx, dy):
+        if torch.is_grad_enabled():
+            refuse_twice("gelu8")
+        k = _unpack_plain(*ctx.saved_tensors, torch.float32).to(
+            torch.float64 if dy.dtype == torch.float64 else torch.float32)
+        return (dy.to(k.dtype) * _gelu_slope(k)).to(dy.dtype)
 
 
 def gelu8(x: torch.Tensor) -> torch.Tensor:
@@ -199,7 +215,7 @@ def gelu8(x: torch.Tensor) -> torch.Tensor:
     _check_input(x, "gelu8")
     native = use_kernels(x, "gelu8")
     if x.requires_grad and torch.is_grad_enabled():
-        return _Gelu8Fn.apply(x, native)
+        return _Gelu8Fn.apply(x) if native else _Gelu8HostFn.apply(x)
     return _gelu_forward(x, False)[0] if native else F.gelu(x)
 
 
@@ -228,12 +244,11 @@ def _dense_grads(dy, codes, scales, want_b: bool, dw=None, db=None, variant: int
                                           variant)
     if ws_bytes < 0:
         raise ValueError(f"dense8: sizes rows={rows}, outputs={N}, inputs={K} are not supported")
-    ws = torch.empty(max(ws_bytes // 4, 1), dtype=torch.float32, device=dev)
+    ws = torch.empty(ws_bytes, dtype=torch.uint8, device=dev)
     with guard(dy):
-        check(L.zk_dense8_wgrad(dy2.data_ptr(), codes.data_ptr(), scales.data_ptr(),
-                                dw.data_ptr(), ptr(db) if want_b else None, ws.data_ptr(),
-                                ws_bytes, rows, N, K, stride, dt, add, variant,
-                                stream_ptr(dev)), "zk_dense8_wgrad")
+        call(L.zk_dense8_wgrad, "zk_dense8_wgrad", dy2.data_ptr(), codes.data_ptr(),
+             scales.data_ptr(), dw.data_ptr(), ptr(db) if want_b else None, ws.data_ptr(),
+             ws_bytes, rows, N, K, stride, dt, add, variant, raw_stream(dev.index))
     return dw, db
 
 
@@ -275,7 +290,8 @@ class _Dense8Fn(torch.autograd.Function):
 
     @staticmethod
     def backward(ctx, dy):
-        once_only("dense8")
+        if torch.is_grad_enabled():
+            refuse_twice("dense8")
         codes, scales, weight = ctx.saved_tensors
         need_x, need_w, need_b = ctx.needs_input_grad
         wp, bp = ctx.weight_param, ctx.bias_param

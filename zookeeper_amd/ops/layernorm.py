@@ -14,82 +14,102 @@ fp32 gradient buffer when the parameter has one
 
 from __future__ import annotations
 
+import functools
 from typing import Optional
 
 import torch
 
-from zookeeper_amd.ops._native import check, direct_grad, grad_ready, lib, stream_ptr
-from zookeeper_amd.ops._rows import (DTYPE_CODES, as_fp32, check_param, guard, once_only, ptr,
-                                     rows_of, use_kernels)
+from zookeeper_amd.ops._native import direct_grad, grad_ready, lib
+from zookeeper_amd.ops._rows import (DTYPE_CODES, as_fp32, call, check_param, guard, ptr,
+                                     raw_stream, refuse_twice, rows_of, use_kernels)
+
+
+@functools.lru_cache(maxsize=256)
+def _ws_bytes(rows: int, cols: int) -> int:
+    return lib().zk_layer_norm_bwd_ws_bytes(rows, cols)
 
 
 def _forward(x, weight, bias, eps: float, stats: bool):
+    """``y``, the rows' mean and rstd ([2, rows] fp32, or None), and what the
+    backward's launch repeats: rows, row stride."""
     x2, rows, stride = rows_of(x)
-    cols = x.shape[-1]
-    y = torch.empty(x.shape, dtype=x.dtype, device=x.device)
-    # [2, rows]: mean, rstd
-    st = torch.empty((2, rows), dtype=torch.float32, device=x.device) if stats else None
-    mean = st.data_ptr() if stats else None
-    rstd = mean + 4 * rows if stats else None
+    dev = x.device
+    y = torch.empty_like(x) if x.is_contiguous() else torch.empty(x.shape, dtype=x.dtype,
+                                                                  device=dev)
+    st = mean = rstd = None
+    if stats:
+        st = torch.empty((2, rows), dtype=torch.float32, device=dev)
+        mean = st.data_ptr()
+        rstd = mean + 4 * rows
+    w, b = as_fp32(weight), as_fp32(bias)
     with guard(x):
-        check(lib().zk_layer_norm_fwd(x2.data_ptr(), ptr(as_fp32(weight)), ptr(as_fp32(bias)),
-                                      y.data_ptr(), mean, rstd, rows, cols, stride,
-                                      eps, DTYPE_CODES[x.dtype], stream_ptr(x.device)),
-              "zk_layer_norm_fwd")
-    return y, st
+        call(lib().zk_layer_norm_fwd, "zk_layer_norm_fwd", x2.data_ptr(), ptr(w), ptr(b),
+             y.data_ptr(), mean, rstd, rows, x.shape[-1], stride, eps, DTYPE_CODES[x.dtype],
+             raw_stream(dev.index))
+    return y, st, rows, stride
 
 
 class _LayerNormFn(torch.autograd.Function):
+    # Small rows wait for this host code and not for the kernels (a backward
+    # runs on a cold thread): everything that the forward knows is passed on.
     @staticmethod
     def forward(ctx, x, weight, bias, eps):
-        y, stats = _forward(x, weight, bias, eps, True)
-        ctx.save_for_backward(x, weight, stats)
+        y, stats, rows, stride = _forward(x, weight, bias, eps, True)
+        ctx.save_for_backward(x, weight)
         # the parameters themselves: the flat gradient buffer hangs on them
-        ctx.weight_param, ctx.bias_param = weight, bias
+        ctx.rest = (stats, rows, stride, weight, bias)
         return y
 
     @staticmethod
     def backward(ctx, dy):
-        once_only("layer_norm")
-        x, weight, stats = ctx.saved_tensors
+        if torch.is_grad_enabled():
+            refuse_twice("layer_norm")
+        x, weight = ctx.saved_tensors
+        stats, rows, stride, wp, bp = ctx.rest
         need_x, need_w, need_b = ctx.needs_input_grad[:3]
-        wp, bp = ctx.weight_param, ctx.bias_param
         dev, cols = x.device, x.shape[-1]
-        dw_direct = direct_grad(wp) if need_w else None
-        db_direct = direct_grad(bp) if need_b else None
-        x2, rows, xs = rows_of(x)
-        dx = torch.empty(x.shape, dtype=x.dtype, device=dev) if need_x else None
-        if rows == 0:
-            dw = torch.zeros_like(wp) if need_w and dw_direct is None else None
-            db = torch.zeros_like(bp) if need_b and db_direct is None else None
+        x2 = x if x.is_contiguous() else rows_of(x)[0]
+        dx = ws = dw = db = dw_direct = db_direct = None
+        add = ws_bytes = 0
+        if dy.is_contiguous():
+            dy2, dys = dy, cols
+            if need_x:
+                dx = torch.empty_like(dy)
         else:
             dy2, _, dys = rows_of(dy)
+            if need_x:
+                dx = torch.empty(x.shape, dtype=x.dtype, device=dev)
+        L = lib()
+        if need_w or need_b:
+            dw_direct = direct_grad(wp) if need_w else None
+            db_direct = direct_grad(bp) if need_b else None
+            new = torch.empty if rows else torch.zeros
             dw, db = dw_direct, db_direct
-            if need_w and dw is None:
-                dw = torch.empty(cols, dtype=torch.float32, device=dev)
-            if need_b and db is None:
-                db = torch.empty(cols, dtype=torch.float32, device=dev)
-            ws, ws_bytes = None, 0
-            if need_w or need_b:
-                ws_bytes = lib().zk_layer_norm_bwd_ws_bytes(rows, cols)
-                ws = torch.empty(ws_bytes // 4, dtype=torch.float32, device=dev)
-            add = (1 if dw_direct is not None else 0) | (2 if db_direct is not None else 0)
-            with guard(x):
-                check(lib().zk_layer_norm_bwd(dy2.data_ptr(), x2.data_ptr(), ptr(as_fp32(weight)),
-                                              stats.data_ptr(), stats.data_ptr() + 4 * rows,
-                                              ptr(dx), ptr(dw),
-                                              ptr(db), ptr(ws), ws_bytes, rows, cols, xs, dys,
-                                              DTYPE_CODES[x.dtype], add, stream_ptr(dev)),
-                      "zk_layer_norm_bwd")
+            if dw is not None:
+                add = 1
+            elif need_w:
+                dw = new(cols, dtype=torch.float32, device=dev)
+            if db is not None:
+                add += 2
+            elif need_b:
+                db = new(cols, dtype=torch.float32, device=dev)
+            ws_bytes = _ws_bytes(rows, cols)
+            ws = torch.empty(ws_bytes, dtype=torch.uint8, device=dev)
+        if rows:
+            mean = stats.data_ptr()
+            w = as_fp32(weight)
+            call(L.zk_layer_norm_bwd, "zk_layer_norm_bwd", dy2.data_ptr(), x2.data_ptr(), ptr(w),
+                 mean, mean + 4 * rows, ptr(dx), ptr(dw), ptr(db), ptr(ws), ws_bytes, rows, cols,
+                 stride, dys, DTYPE_CODES[x.dtype], add, raw_stream(dev.index))
         if dw_direct is not None:
             grad_ready(wp)
             dw = None
-        elif dw is not None and dw.dtype != wp.dtype:
+        elif dw is not None and wp.dtype != torch.float32:
             dw = dw.to(wp.dtype)
         if db_direct is not None:
             grad_ready(bp)
             db = None
-        elif db is not None and db.dtype != bp.dtype:
+        elif db is not None and bp.dtype != torch.float32:
             db = db.to(bp.dtype)
         return dx, dw, db, None
 

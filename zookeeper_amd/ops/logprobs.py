@@ -25,8 +25,9 @@ from typing import NamedTuple, Optional
 
 import torch
 
-from zookeeper_amd.ops._native import check, lib, stream_ptr
-from zookeeper_amd.ops._rows import DTYPE_CODES, guard, once_only, ptr, rows_of, use_kernels
+from zookeeper_amd.ops._native import lib
+from zookeeper_amd.ops._rows import (DTYPE_CODES, call, guard, ptr, raw_stream, refuse_twice,
+                                     rows_of, use_kernels)
 
 MAX_TOP = 64
 
@@ -52,46 +53,49 @@ def _forward(logits, tokens, top: int, ignore: int, keep: bool):
         top_ids = torch.empty((*lead, top), dtype=torch.int64, device=dev)
     ws_bytes = L.zk_token_logprobs_ws_bytes(rows, V, top)
     if ws_bytes:
-        ws = torch.empty(ws_bytes // 8, dtype=torch.int64, device=dev)
+        ws = torch.empty(ws_bytes, dtype=torch.uint8, device=dev)
     with guard(logits):
-        check(L.zk_token_logprobs_fwd(x.data_ptr(), tokens.data_ptr(), logp.data_ptr(),
-                                      entropy.data_ptr(), ptr(stats), ptr(top_logp), ptr(top_ids),
-                                      ptr(ws), ws_bytes, rows, V, stride, top, ignore,
-                                      DTYPE_CODES[logits.dtype], stream_ptr(dev)),
-              "zk_token_logprobs_fwd")
-    return logp, entropy, top_logp, top_ids, stats
+        call(L.zk_token_logprobs_fwd, "zk_token_logprobs_fwd", x.data_ptr(), tokens.data_ptr(),
+             logp.data_ptr(), entropy.data_ptr(), ptr(stats), ptr(top_logp), ptr(top_ids),
+             ptr(ws), ws_bytes, rows, V, stride, top, ignore, DTYPE_CODES[logits.dtype],
+             raw_stream(dev.index))
+    return logp, entropy, top_logp, top_ids, stats, rows, stride
 
 
 class _TokenLogProbsFn(torch.autograd.Function):
     @staticmethod
     def forward(ctx, logits, tokens, top, ignore):
-        logp, entropy, top_logp, top_ids, stats = _forward(logits, tokens, top, ignore, True)
-        ctx.save_for_backward(logits, tokens, stats)
-        ctx.ignore = ignore
+        (logp, entropy, top_logp, top_ids, stats, rows,
+         stride) = _forward(logits, tokens, top, ignore, True)
+        ctx.save_for_backward(logits, tokens)
+        ctx.rest = (stats, rows, stride, ignore)
         ctx.set_materialize_grads(False)
         if top:
             ctx.mark_non_differentiable(top_logp, top_ids)
-        return logp, entropy, top_logp, top_ids
+            return logp, entropy, top_logp, top_ids
+        return logp, entropy
 
     @staticmethod
-    def backward(ctx, g_logp, g_entropy, _g_top, _g_ids):
-        once_only("token_logprobs")
+    def backward(ctx, g_logp, g_entropy, *_):
+        if torch.is_grad_enabled():
+            refuse_twice("token_logprobs")
         if g_logp is None and g_entropy is None:
             return None, None, None, None
-        logits, tokens, stats = ctx.saved_tensors
-        x, rows, stride = rows_of(logits)
-        dev = logits.device
-        dx = torch.empty(logits.shape, dtype=logits.dtype, device=dev)
-        if g_logp is not None:
+        logits, tokens = ctx.saved_tensors
+        stats, rows, stride, ignore = ctx.rest
+        if logits.is_contiguous():
+            x, dx = logits, torch.empty_like(logits)
+        else:
+            x = rows_of(logits)[0]
+            dx = torch.empty(logits.shape, dtype=logits.dtype, device=logits.device)
+        if g_logp is not None and not g_logp.is_contiguous():
             g_logp = g_logp.contiguous()
-        if g_entropy is not None:
+        if g_entropy is not None and not g_entropy.is_contiguous():
             g_entropy = g_entropy.contiguous()
-        with guard(logits):
-            check(lib().zk_token_logprobs_bwd(x.data_ptr(), tokens.data_ptr(), stats.data_ptr(),
-                                              ptr(g_logp), ptr(g_entropy), dx.data_ptr(), rows,
-                                              logits.shape[-1], stride, ctx.ignore,
-                                              DTYPE_CODES[logits.dtype], stream_ptr(dev)),
-                  "zk_token_logprobs_bwd")
+        call(lib().zk_token_logprobs_bwd, "zk_token_logprobs_bwd", x.data_ptr(),
+             tokens.data_ptr(), stats.data_ptr(), ptr(g_logp), ptr(g_entropy), dx.data_ptr(),
+             rows, logits.shape[-1], stride, ignore, DTYPE_CODES[logits.dtype],
+             raw_stream(logits.device.index))
         return dx, None, None, None
 
 
