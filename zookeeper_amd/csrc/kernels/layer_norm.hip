@@ -23,8 +23,10 @@
 
 namespace {
 
-constexpr int kNT = 256;       // threads per block
+constexpr int kNT = 256;       // threads per block (rows of G > 256 lanes: G)
 constexpr int kMaxD = 16384;   // widest row kept in registers
+
+constexpr int block_of(int g) { return g > kNT ? g : kNT; }
 
 struct LnArgs {
   const void* x;       // [rows][xs]
@@ -40,17 +42,20 @@ struct LnArgs {
   float eps;
 };
 
-// G lanes per row (<= 64: groups inside a wave; 256: the block)
+// Sums over the G lanes of a row: groups inside a wave, or a block of G / 64 waves
+// (red: 2 * G / 64 floats that nobody reads any more).
 template <int G>
 __device__ __forceinline__ float row_sum(float v, float* red) {
   if constexpr (G <= 64) {
     return group_sum<G>(v);
   } else {
     v = group_sum<64>(v);
-    __syncthreads();  // the previous use of red has been read
     if ((threadIdx.x & 63) == 0) red[threadIdx.x >> 6] = v;
     __syncthreads();
-    return (red[0] + red[1]) + (red[2] + red[3]);
+    float s = red[0];
+#pragma unroll
+    for (int i = 1; i < G / 64; ++i) s += red[i];
+    return s;
   }
 }
 
@@ -60,16 +65,21 @@ __device__ __forceinline__ void row_sum2(float& a, float& b, float* red) {
     a = group_sum<G>(a);
     b = group_sum<G>(b);
   } else {
+    constexpr int W = G / 64;
     a = group_sum<64>(a);
     b = group_sum<64>(b);
-    __syncthreads();
     if ((threadIdx.x & 63) == 0) {
       red[threadIdx.x >> 6] = a;
-      red[4 + (threadIdx.x >> 6)] = b;
+      red[W + (threadIdx.x >> 6)] = b;
     }
     __syncthreads();
-    a = (red[0] + red[1]) + (red[2] + red[3]);
-    b = (red[4] + red[5]) + (red[6] + red[7]);
+    a = red[0];
+    b = red[W];
+#pragma unroll
+    for (int i = 1; i < W; ++i) {
+      a += red[i];
+      b += red[W + i];
+    }
   }
 }
 
@@ -84,12 +94,12 @@ __device__ __forceinline__ void load_param(const float* p, int c, int n, float f
 }
 
 template <int DT, int G, int NV>
-__global__ __launch_bounds__(kNT) void ln_fwd_kernel(LnArgs a) {
+__global__ __launch_bounds__(block_of(G)) void ln_fwd_kernel(LnArgs a) {
   typedef typename Elem<DT>::raw raw;
-  __shared__ float red[8];
+  __shared__ float red[2][16];
   const int l = threadIdx.x % G;
-  const long long row = a.row0 + (long long)blockIdx.x * (kNT / G) + threadIdx.x / G;
-  if (row >= a.rows) return;  // G = 256: never (one row per block)
+  const long long row = a.row0 + (long long)blockIdx.x * (block_of(G) / G) + threadIdx.x / G;
+  if (row >= a.rows) return;  // G >= 256: never (one row per block)
   const raw* x = reinterpret_cast<const raw*>(a.x) + row * a.xs;
   raw* y = reinterpret_cast<raw*>(a.out) + row * a.D;
   float v[NV][8];
@@ -102,7 +112,7 @@ __global__ __launch_bounds__(kNT) void ln_fwd_kernel(LnArgs a) {
     for (int i = 0; i < 8; ++i) s += v[k][i];
   }
   const float invd = 1.f / (float)a.D;
-  const float mean = row_sum<G>(s, red) * invd;
+  const float mean = row_sum<G>(s, red[0]) * invd;
   float q = 0.f;
 #pragma unroll
   for (int k = 0; k < NV; ++k) {
@@ -113,7 +123,7 @@ __global__ __launch_bounds__(kNT) void ln_fwd_kernel(LnArgs a) {
       if (i < n) q += v[k][i] * v[k][i];
     }
   }
-  const float rstd = rsqrtf(row_sum<G>(q, red) * invd + a.eps);
+  const float rstd = rsqrtf(row_sum<G>(q, red[1]) * invd + a.eps);
 #pragma unroll
   for (int k = 0; k < NV; ++k) {
     const int c = (k * G + l) * 8, n = a.D - c;
@@ -136,7 +146,7 @@ __global__ __launch_bounds__(kNT) void ln_fwd_kernel(LnArgs a) {
 template <int DT>
 __global__ __launch_bounds__(kNT) void ln_fwd_loop_kernel(LnArgs a) {
   typedef typename Elem<DT>::raw raw;
-  __shared__ float red[8];
+  __shared__ float red[2][16];
   const long long row = a.row0 + blockIdx.x;
   const raw* x = reinterpret_cast<const raw*>(a.x) + row * a.xs;
   raw* y = reinterpret_cast<raw*>(a.out) + row * a.D;
@@ -147,13 +157,13 @@ __global__ __launch_bounds__(kNT) void ln_fwd_loop_kernel(LnArgs a) {
 #pragma unroll
     for (int i = 0; i < 8; ++i) s += f[i];
   }
-  const float mean = row_sum<kNT>(s, red) * invd;
+  const float mean = row_sum<kNT>(s, red[0]) * invd;
   for (long long c = threadIdx.x * 8; c < a.D; c += kNT * 8) {
     load8_n<DT>(x + c, (int)min(8LL, a.D - c), mean, f);
 #pragma unroll
     for (int i = 0; i < 8; ++i) q += (f[i] - mean) * (f[i] - mean);
   }
-  const float rstd = rsqrtf(row_sum<kNT>(q, red) * invd + a.eps);
+  const float rstd = rsqrtf(row_sum<kNT>(q, red[1]) * invd + a.eps);
   for (long long c = threadIdx.x * 8; c < a.D; c += kNT * 8) {
     const int n = (int)min(8LL, a.D - c);
     float w[8], b[8];
@@ -170,12 +180,15 @@ __global__ __launch_bounds__(kNT) void ln_fwd_loop_kernel(LnArgs a) {
   }
 }
 
-// Blocks walk the rows; a lane group keeps the sums of its columns.
+// Blocks walk the rows; a lane group keeps the sums of its columns.  The next row's
+// loads are in flight while a row is reduced and written (without them bf16 rows
+// ran at 3.1 TB/s: too few bytes in flight, 32768 x 2048 112 us).
 template <int DT, int G, int NV>
-__global__ __launch_bounds__(kNT) void ln_bwd_kernel(LnArgs a) {
+__global__ __launch_bounds__(block_of(G)) void ln_bwd_kernel(LnArgs a) {
   typedef typename Elem<DT>::raw raw;
-  __shared__ float red[8];
-  constexpr int RPB = kNT / G;  // rows of a block at a time
+  constexpr int NT = block_of(G), RPB = NT / G;  // RPB: rows of a block at a time
+  constexpr bool AHEAD = G < 1024;  // 16 waves leave 128 registers each: none to spare
+  __shared__ float red[2][32];
   const int l = threadIdx.x % G, grp = threadIdx.x / G;
   const float invd = 1.f / (float)a.D;
   float w[NV][8], dw[NV][8], db[NV][8];
@@ -186,20 +199,38 @@ __global__ __launch_bounds__(kNT) void ln_bwd_kernel(LnArgs a) {
 #pragma unroll
     for (int i = 0; i < 8; ++i) dw[k][i] = db[k][i] = 0.f;
   }
-  // G = 256: the trip count is the same for the whole block (row_sum's barriers)
-  for (long long row = (long long)blockIdx.x * RPB + grp; row < a.rows;
-       row += (long long)gridDim.x * RPB) {
-    const raw* x = reinterpret_cast<const raw*>(a.x) + row * a.xs;
-    const raw* dy = reinterpret_cast<const raw*>(a.dy) + row * a.dys;
-    const float mean = a.mean[row], rstd = a.rstd[row];
-    float xh[NV][8], g[NV][8];
-    float s1 = 0.f, s2 = 0.f;
+  const long long stride = (long long)gridDim.x * RPB;
+  long long row = (long long)blockIdx.x * RPB + grp;
+  Raw8<DT> nx[NV], ny[NV];
+  float nm = 0.f, nr = 0.f;
+  auto load = [&](long long r) {
+    const raw* x = reinterpret_cast<const raw*>(a.x) + r * a.xs;
+    const raw* dy = reinterpret_cast<const raw*>(a.dy) + r * a.dys;
 #pragma unroll
     for (int k = 0; k < NV; ++k) {
       const int c = (k * G + l) * 8;
-      load8_n<DT>(x + c, a.D - c, mean, xh[k]);
-      load8_n<DT>(dy + c, a.D - c, 0.f, g[k]);
+      nx[k] = raw8<DT>(x + c, a.D - c);
+      ny[k] = raw8<DT>(dy + c, a.D - c);  // zeros behind D: no share in any sum
     }
+    nm = a.mean[r];
+    nr = a.rstd[r];
+  };
+  if (AHEAD && row < a.rows) load(row);
+  // G > 64: the trip count is the same for the whole block (row_sum2's barrier; its
+  // buffers alternate, so one barrier per row is enough)
+  for (int it = 0; row < a.rows; row += stride, it ^= 1) {
+    if (!AHEAD) load(row);
+    float xh[NV][8], g[NV][8];
+#pragma unroll
+    for (int k = 0; k < NV; ++k)
+#pragma unroll
+      for (int i = 0; i < 8; ++i) {
+        xh[k][i] = raw_at<DT>(nx[k], i);
+        g[k][i] = raw_at<DT>(ny[k], i);
+      }
+    const float mean = nm, rstd = nr;
+    if (AHEAD && row + stride < a.rows) load(row + stride);
+    float s1 = 0.f, s2 = 0.f;
 #pragma unroll
     for (int k = 0; k < NV; ++k)
 #pragma unroll
@@ -214,7 +245,7 @@ __global__ __launch_bounds__(kNT) void ln_bwd_kernel(LnArgs a) {
         g[k][i] = gw;
       }
     if (a.out) {
-      row_sum2<G>(s1, s2, red);
+      row_sum2<G>(s1, s2, red[it]);
       s1 *= invd;
       s2 *= invd;
       raw* dx = reinterpret_cast<raw*>(a.out) + row * a.D;
@@ -358,8 +389,18 @@ __global__ __launch_bounds__(1024) void ln_part_sum_kernel(const float* __restri
   const long long n2 = 2LL * D;
   const long long c = (long long)blockIdx.x * 64 + col;
   float s = 0.f;
-  if (c < n2)
-    for (int p = sl; p < parts; p += 16) s += part[(long long)p * n2 + c];
+  if (c < n2) {
+    const float* p = part + sl * n2 + c;
+    int k = sl;
+    for (; k + 112 < parts; k += 128, p += 128 * n2) {  // eight loads in flight
+      float v[8];
+#pragma unroll
+      for (int i = 0; i < 8; ++i) v[i] = p[16 * i * n2];
+#pragma unroll
+      for (int i = 0; i < 8; ++i) s += v[i];
+    }
+    for (; k < parts; k += 16, p += 16 * n2) s += *p;
+  }
   red[sl][col] = s;
   __syncthreads();
   if (sl == 0 && c < n2) {
@@ -373,41 +414,60 @@ __global__ __launch_bounds__(1024) void ln_part_sum_kernel(const float* __restri
   }
 }
 
-// Blocks of the backward: enough that the partials are few next to the rows
-// and every CU has work.
+// Lanes and vectors of a row by its length: at most two vectors per lane (the
+// backward holds 40 registers for each), few idle lanes.
+#define ZK_LN_SHAPES(D, RUN)      \
+  do {                            \
+    if ((D) <= 8) RUN(1, 1);      \
+    else if ((D) <= 16) RUN(2, 1);   \
+    else if ((D) <= 32) RUN(4, 1);   \
+    else if ((D) <= 64) RUN(8, 1);   \
+    else if ((D) <= 128) RUN(16, 1); \
+    else if ((D) <= 256) RUN(32, 1); \
+    else if ((D) <= 512) RUN(64, 1); \
+    else if ((D) <= 1024) RUN(64, 2);   \
+    else if ((D) <= 2048) RUN(256, 1);  \
+    else if ((D) <= 4096) RUN(256, 2);  \
+    else if ((D) <= 8192) RUN(512, 2);  \
+    else RUN(1024, 2);               \
+  } while (0)
+
+// Blocks of the backward: as many as the chip holds at a time, but each lane group
+// has at least four rows (its partial sums are two fp32 rows to write and read
+// again), if that leaves 64 blocks.
 int bwd_blocks(long long rows, int D) {
-  long long rpb = 1;
-  if (D <= 32) rpb = 64;
-  else if (D <= 128) rpb = 16;
-  else if (D <= 2048) rpb = 4;
-  long long nb = (rows + rpb - 1) / rpb;
-  const long long cap = 512;
-  return (int)(nb < cap ? nb : cap);
+  long long rpb = 1, cap = 1024;
+#define ZK_LN_RPB(G, NV)            \
+  do {                              \
+    rpb = block_of(G) / G;          \
+    cap = 1024 / (block_of(G) / kNT); \
+  } while (0)
+  ZK_LN_SHAPES(D, ZK_LN_RPB);
+#undef ZK_LN_RPB
+  const long long all = (rows + rpb - 1) / rpb;
+  long long nb = rows / (4 * rpb);
+  if (nb < 64) nb = 64;
+  if (nb > cap) nb = cap;
+  return (int)(nb < all ? nb : all);
 }
 
 int loop_parts(long long rows) { return (int)(rows < 64 ? rows : 64); }
 
 // Rows of one launch of the kernels that give a row to a block: a grid holds
 // fewer than 2^32 threads.
-constexpr long long kRowsPerLaunch = 1LL << 23;
+constexpr long long kRowsPerLaunch = 1LL << 21;
 
 template <int DT>
 int fwd_dispatch(LnArgs a, hipStream_t st) {
   for (a.row0 = 0; a.row0 < a.rows; a.row0 += kRowsPerLaunch) {
     const long long left = a.rows - a.row0;
     const unsigned r = (unsigned)(left < kRowsPerLaunch ? left : kRowsPerLaunch);
-#define ZK_LN_FWD(G, NV)                                                                       \
-  hipLaunchKernelGGL((ln_fwd_kernel<DT, G, NV>), dim3((r + kNT / G - 1) / (kNT / G)), dim3(kNT), \
+#define ZK_LN_FWD(G, NV)                                                                    \
+  hipLaunchKernelGGL((ln_fwd_kernel<DT, G, NV>),                                            \
+                     dim3((r + block_of(G) / G - 1) / (block_of(G) / G)), dim3(block_of(G)), \
                      0, st, a)
-  if (a.D <= 32) ZK_LN_FWD(4, 1);
-  else if (a.D <= 128) ZK_LN_FWD(16, 1);
-  else if (a.D <= 512) ZK_LN_FWD(64, 1);
-  else if (a.D <= 1024) ZK_LN_FWD(64, 2);
-  else if (a.D <= 2048) ZK_LN_FWD(256, 1);
-  else if (a.D <= 4096) ZK_LN_FWD(256, 2);
-  else if (a.D <= 8192) ZK_LN_FWD(256, 4);
-  else if (a.D <= kMaxD) ZK_LN_FWD(256, 8);
-  else hipLaunchKernelGGL(ln_fwd_loop_kernel<DT>, dim3(r), dim3(kNT), 0, st, a);
+    if (a.D > kMaxD) hipLaunchKernelGGL(ln_fwd_loop_kernel<DT>, dim3(r), dim3(kNT), 0, st, a);
+    else ZK_LN_SHAPES(a.D, ZK_LN_FWD);
 #undef ZK_LN_FWD
     ZK_CHECK_LAUNCH();
   }
@@ -416,16 +476,9 @@ int fwd_dispatch(LnArgs a, hipStream_t st) {
 
 template <int DT>
 int bwd_dispatch(const LnArgs& a, int blocks, hipStream_t st) {
-#define ZK_LN_BWD(G, NV) \
-  hipLaunchKernelGGL((ln_bwd_kernel<DT, G, NV>), dim3(blocks), dim3(kNT), 0, st, a)
-  if (a.D <= 32) ZK_LN_BWD(4, 1);
-  else if (a.D <= 128) ZK_LN_BWD(16, 1);
-  else if (a.D <= 512) ZK_LN_BWD(64, 1);
-  else if (a.D <= 1024) ZK_LN_BWD(64, 2);
-  else if (a.D <= 2048) ZK_LN_BWD(64, 4);
-  else if (a.D <= 4096) ZK_LN_BWD(256, 2);
-  else if (a.D <= 8192) ZK_LN_BWD(256, 4);
-  else if (a.D <= kMaxD) ZK_LN_BWD(256, 8);
+#define ZK_LN_BWD(G, NV)                                                                     \
+  hipLaunchKernelGGL((ln_bwd_kernel<DT, G, NV>), dim3(blocks), dim3(block_of(G)), 0, st, a)
+  ZK_LN_SHAPES(a.D, ZK_LN_BWD);
 #undef ZK_LN_BWD
   return (int)hipGetLastError();
 }

@@ -42,6 +42,48 @@ struct Elem<2> {
 typedef uint32_t Bytes16 __attribute__((ext_vector_type(4), aligned(1)));
 typedef uint32_t Bytes8 __attribute__((ext_vector_type(2), aligned(1)));
 
+// 8 elements as loaded (a row in flight takes half the registers in 16 bits).
+template <int DT>
+struct Raw8 {
+  uint32_t v[DT == 0 ? 8 : 4];
+};
+
+// the first n (<= 8; may be negative) elements, zeros behind them
+template <int DT>
+__device__ __forceinline__ Raw8<DT> raw8(const typename Elem<DT>::raw* p, int n) {
+  Raw8<DT> r;
+  if (n >= 8) {
+    const Bytes16 a = *reinterpret_cast<const Bytes16*>(p);
+#pragma unroll
+    for (int i = 0; i < 4; ++i) r.v[i] = a[i];
+    if constexpr (DT == 0) {
+      const Bytes16 b = *reinterpret_cast<const Bytes16*>(p + 4);
+#pragma unroll
+      for (int i = 0; i < 4; ++i) r.v[4 + i] = b[i];
+    }
+  } else {
+#pragma unroll
+    for (int i = 0; i < (DT == 0 ? 8 : 4); ++i) {
+      if constexpr (DT == 0) {
+        r.v[i] = i < n ? __float_as_uint(p[i]) : 0u;
+      } else {
+        r.v[i] = (2 * i < n ? (uint32_t)p[2 * i] : 0u) |
+                 (2 * i + 1 < n ? (uint32_t)p[2 * i + 1] << 16 : 0u);
+      }
+    }
+  }
+  return r;
+}
+
+template <int DT>
+__device__ __forceinline__ float raw_at(const Raw8<DT>& r, int i) {
+  if constexpr (DT == 0) {
+    return __uint_as_float(r.v[i]);
+  } else {
+    return Elem<DT>::up((uint16_t)(r.v[i >> 1] >> (16 * (i & 1))));
+  }
+}
+
 template <int DT>
 __device__ __forceinline__ void load8(const typename Elem<DT>::raw* p, float (&f)[8]) {
   if constexpr (DT == 0) {
