@@ -851,6 +851,9 @@ D8Plan dense8_plan(long long M, int N, int K, int dt, long long dys, bool aligne
         s = c;
       }
     }
+#ifdef FS
+    s = FS;
+#endif
     p.rps = ((R + s - 1) / s + 63) / 64 * 64;
     p.splits = (int)((R + p.rps - 1) / p.rps);
   } else {

@@ -20,12 +20,17 @@
 // Top k: a wave holds its k best keys sorted, one per lane.  A key is the
 // order-preserving image of the value with the complement of the place under
 // it, so equal values rank by the lower place and no two keys are equal.
-// Values above the k-th key (a compare per element, nearly always false) are
-// collected in LDS, up to 64, and merged by rank: a key's place is the number
-// of greater ones.  When one 512-element tile has more candidates than the
-// buffer takes, the k-th largest of its lane maxima (a binary search with
-// ballots) raises the threshold first, so a rising row costs a merge per tile
-// and not one per element.
+// A tile of 512 elements is passed over when its lanes' maxima (which the running
+// statistics need anyway) stay at or under the k-th value.  Else its greater values
+// are collected in LDS, up to 64, and merged by rank: a key's place is the number of
+// greater ones.  When a tile has more candidates than the buffer takes, the k-th
+// largest of its lane maxima (a binary search with ballots) raises the threshold
+// first, so a rising row costs a merge per tile and not one per element.
+//
+// Joining lists (of the waves of a block, of the splits of a row): with j = ceil(k /
+// lists), the ceil(k / j)-th largest of the lists' j-th keys has at least k keys at or
+// above it; only those are merged, some 1.5 k of a list each times k.  (Merging list
+// by list instead took 30 of the 36 us of one row of 129000 with k = 20.)
 //
 // Rows: all -inf -> logp -inf, entropy 0, gradient 0.  A NaN or +inf -> NaN.
 // The ignored index: logp 0 and no gradient from it.  Any other token outside
@@ -49,9 +54,16 @@ struct Stat {
   float m, s, q;
 };
 
-__device__ __forceinline__ void stat_add8(Stat& a, const float (&x)[8]) {
-  const float v = fmaxf(fmaxf(fmaxf(x[0], x[1]), fmaxf(x[2], x[3])),
-                        fmaxf(fmaxf(x[4], x[5]), fmaxf(x[6], x[7])));
+// the greatest of 8; NaN if one is
+__device__ __forceinline__ float max8(const float (&x)[8]) {
+  float v = x[0];
+#pragma unroll
+  for (int i = 1; i < 8; ++i) v = __builtin_elementwise_maximum(v, x[i]);
+  return v;
+}
+
+// v: max8(x).  A NaN reaches s through its own term, so m may drop it.
+__device__ __forceinline__ void stat_add8(Stat& a, const float (&x)[8], float v) {
   const float m = fmaxf(a.m, v);
   const float ms = m == -INFINITY ? 0.f : m;
   const float d0 = a.m - ms, c = exp_d(d0);
@@ -113,77 +125,102 @@ __device__ __forceinline__ void wave_fence() {
 struct Top {
   u64 best;   // lane i: the i-th greatest key so far (0: none)
   u64 least;  // a key must exceed this one to matter (wave-uniform)
+  float thr;  // ... as a value; NaN while anything may enter
   int fill;   // keys waiting in buf (wave-uniform)
   int k;
   u64* buf;   // LDS: 64 waiting keys
-  u64* tmp;   // LDS: 64 slots of the merge
+  u64* lst;   // LDS: 64 slots of the merge
 };
 
-// Merge lane i's key `b` (i < n) into the sorted list.
-__device__ __forceinline__ void top_merge(Top& t, u64 b, int n) {
-  const int lane = threadIdx.x & 63;
-  b = lane < n ? b : 0;
-  int rl = lane, rb = 0;  // the list is sorted: its own greater keys are the lanes below
-  for (int i = 0; i < n; ++i) {
-    const u64 o = lane64(b, i);
-    rl += o > t.best;
-    rb += o > b;
+__device__ __forceinline__ Top top_new(int k, u64* lds) {
+  return Top{0, 0, NAN, 0, k, lds, lds + 64};
+}
+
+__device__ __forceinline__ void top_raise(Top& t, u64 least) {
+  if (least > t.least) {
+    t.least = least;
+    t.thr = value_of((uint32_t)(least >> 32));
   }
-  for (int i = 0; i < t.k; ++i) rb += lane64(t.best, i) > b;
-  t.tmp[lane] = 0;
+}
+
+// Merge the n keys in buf (any order) into the sorted list.
+__device__ __forceinline__ void top_merge(Top& t, int n) {
+  typedef u64 u64x2 __attribute__((ext_vector_type(2)));
+  const int lane = threadIdx.x & 63;
+  if (lane >= n) t.buf[lane] = 0;
+  t.lst[lane] = t.best;
   wave_fence();
-  if (t.best != 0 && rl < t.k) t.tmp[rl] = t.best;
-  if (b != 0 && rb < t.k) t.tmp[rb] = b;
+  const u64 b = t.buf[lane];
+  int rl = lane, rb = 0;  // the list is sorted: its own greater keys are the lanes below
+  for (int i = 0; i < n; i += 4) {
+    const u64x2 p = *reinterpret_cast<const u64x2*>(t.buf + i);
+    const u64x2 q = *reinterpret_cast<const u64x2*>(t.buf + i + 2);
+    rl += (p[0] > t.best) + (p[1] > t.best) + (q[0] > t.best) + (q[1] > t.best);
+    rb += (p[0] > b) + (p[1] > b) + (q[0] > b) + (q[1] > b);
+  }
+  if (lane64(t.best, 0) != 0) {
+    for (int i = 0; i < t.k; i += 4) {  // behind k: zeros
+      const u64x2 p = *reinterpret_cast<const u64x2*>(t.lst + i);
+      const u64x2 q = *reinterpret_cast<const u64x2*>(t.lst + i + 2);
+      rb += (p[0] > b) + (p[1] > b) + (q[0] > b) + (q[1] > b);
+    }
+  }
   wave_fence();
-  t.best = t.tmp[lane];
+  t.lst[lane] = 0;
   wave_fence();
-  const u64 last = lane64(t.best, t.k - 1);
-  t.least = last > t.least ? last : t.least;
+  if (t.best != 0 && rl < t.k) t.lst[rl] = t.best;
+  if (b != 0 && rb < t.k) t.lst[rb] = b;
+  wave_fence();
+  t.best = t.lst[lane];
+  wave_fence();
+  top_raise(t, lane64(t.best, t.k - 1));
 }
 
 __device__ __forceinline__ void top_flush(Top& t) {
   if (t.fill == 0) return;
   wave_fence();
-  const u64 b = t.buf[threadIdx.x & 63];
-  top_merge(t, b, t.fill);
+  top_merge(t, t.fill);
   t.fill = 0;
 }
 
-// Eight elements per lane, places base .. base + n - 1; places rise from tile
-// to tile of a wave, so a value equal to the list's last never enters later.
-__device__ __forceinline__ void top_add8(Top& t, const float (&x)[8], int base, int n) {
+// One key per lane (0: none) into the waiting ones.
+__device__ __forceinline__ void top_push(Top& t, u64 key) {
+  u64 in = __ballot(key > t.least);
+  if (in == 0) return;
+  if (t.fill + __popcll(in) > 64) {
+    top_flush(t);
+    in = __ballot(key > t.least);
+  }
+  const int at = t.fill + __builtin_amdgcn_mbcnt_hi((uint32_t)(in >> 32),
+                                                    __builtin_amdgcn_mbcnt_lo((uint32_t)in, 0));
+  if (key > t.least) t.buf[at] = key;
+  t.fill += __popcll(in);
+}
+
+// Eight elements per lane, places base .. base + n - 1, v = max8 of them; places
+// rise from tile to tile of a wave, so a value equal to the list's last never enters
+// later.
+__device__ __forceinline__ void top_add8(Top& t, const float (&x)[8], float v, int base, int n) {
+  if (__ballot(!(v <= t.thr)) == 0) return;
   uint32_t o[8], top = 0;
 #pragma unroll
   for (int j = 0; j < 8; ++j) {
     o[j] = j < n ? order_of(x[j]) : 0u;
     top = o[j] > top ? o[j] : top;
   }
-  uint32_t least = (uint32_t)(t.least >> 32);
-  if (__ballot(top > least) == 0) return;
-  int count = 0;
-#pragma unroll
-  for (int j = 0; j < 8; ++j) count += __popcll(__ballot(o[j] > least));
-  if (t.fill + count > 64) {
-    // at least k values of this tile are >= the k-th largest lane maximum
+  // many lanes with a candidate: at least k values of this tile are >= the k-th
+  // largest lane maximum
+  if (__popcll(__ballot(top > (uint32_t)(t.least >> 32))) > 24) {
     uint32_t kth = 0;
     for (uint32_t bit = 0x80000000u; bit >= 0x10000u; bit >>= 1)
       if (__popcll(__ballot(top >= (kth | bit))) >= t.k) kth |= bit;
-    if (kth > least) t.least = ((u64)(kth - 1) << 32) | 0xffffffffull;
+    if (kth > 0) top_raise(t, ((u64)(kth - 1) << 32) | 0xffffffffull);
   }
 #pragma unroll
-  for (int j = 0; j < 8; ++j) {
-    const u64 key = o[j] ? ((u64)o[j] << 32) | (uint32_t)~(uint32_t)(base + j) : 0;
-    u64 in = __ballot(key > t.least);
-    if (in == 0) continue;
-    if (t.fill + __popcll(in) > 64) {
-      top_flush(t);
-      in = __ballot(key > t.least);
-    }
-    const int at = t.fill + __builtin_amdgcn_mbcnt_hi((uint32_t)(in >> 32),
-                                                      __builtin_amdgcn_mbcnt_lo((uint32_t)in, 0));
-    if (key > t.least) t.buf[at] = key;
-    t.fill += __popcll(in);
-  }
+  for (int j = 0; j < 8; ++j)
+    top_push(t, o[j] ? ((u64)o[j] << 32) | (uint32_t)~(uint32_t)(base + j) : 0);
+  // a merge lowers the number of later tiles that get here
+  if (t.fill >= 16 || t.fill >= t.k) top_flush(t);
 }
 
 struct LpArgs {
@@ -195,7 +232,7 @@ struct LpArgs {
   float* top_logp;          // [rows][k]
   long long* top_ids;       // [rows][k]
   float* pstat;             // [rows][splits][4]
-  u64* pkeys;               // [rows][splits][k]
+  u64* pkeys;               // [rows][splits * 4][k]: a list per wave
   const float* g_logp;      // backward: [rows] or null
   const float* g_entropy;   // [rows] or null
   void* dx;                 // [rows][V]
@@ -241,11 +278,14 @@ __device__ __forceinline__ void top_write(const LpArgs& a, long long row, u64 ke
   }
 }
 
-// WPR waves per row and split: 1 (four rows per block) or 4 (the block).
+// WPR waves per row and split: 1 (four rows per block) or 4 (the block).  Eight waves
+// per SIMD: with the 110 registers that the filter would take, 4095 x 50001, k = 5
+// ran 160 us instead of 124.
 template <int DT, bool TOP, int WPR>
-__global__ __launch_bounds__(kNT) void lp_fwd_kernel(LpArgs a) {
+__global__ __launch_bounds__(kNT, 8) void lp_fwd_kernel(LpArgs a) {
   typedef typename Elem<DT>::raw raw;
-  __shared__ u64 lds[TOP ? 4 * 128 : 1];
+  __shared__ __attribute__((aligned(16))) u64 lds[TOP ? 4 * 128 : 1];
+  __shared__ u64 keys[TOP && WPR == 4 ? 4 * 64 : 1];
   __shared__ Stat joined[4];
   const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63;
   const long long unit = WPR == 1 ? (long long)blockIdx.x * 4 + wave : blockIdx.x;
@@ -255,43 +295,59 @@ __global__ __launch_bounds__(kNT) void lp_fwd_kernel(LpArgs a) {
   const int lo = split * a.chunk, hi = min(a.V, lo + a.chunk);
   const raw* x = reinterpret_cast<const raw*>(a.x) + row * a.xs;
   Stat st{-INFINITY, 0.f, 0.f};
-  Top top{0, 0, 0, a.k, lds + (TOP ? wave * 128 : 0), lds + (TOP ? wave * 128 + 64 : 0)};
+  Top top = top_new(a.k, lds + (TOP ? wave * 128 : 0));
   const int w = WPR == 1 ? 0 : wave;
-  for (int c0 = lo + w * 512; c0 < hi; c0 += WPR * 512) {  // wave-uniform
-    const int c = c0 + lane * 8;
+  int c0 = lo + w * 512;
+  Raw8<DT> next = raw8<DT>(x + c0 + lane * 8, hi - c0 - lane * 8);
+  for (; c0 < hi; c0 += WPR * 512) {  // wave-uniform
+    const int c = c0 + lane * 8, cn = c + WPR * 512;
     float f[8];
-    load8_n<DT>(x + c, hi - c, -INFINITY, f);
-    stat_add8(st, f);
-    if constexpr (TOP) top_add8(top, f, c, hi - c);
+#pragma unroll
+    for (int i = 0; i < 8; ++i) f[i] = raw_at<DT>(next, i);
+    next = raw8<DT>(x + cn, hi - cn);
+    if (hi - c < 8) {
+#pragma unroll
+      for (int i = 0; i < 8; ++i)
+        if (i >= hi - c) f[i] = -INFINITY;
+    }
+    const float v = max8(f);
+    stat_add8(st, f, v);
+    if constexpr (TOP) top_add8(top, f, v, c, hi - c);
   }
   st = stat_wave(st);
   if constexpr (TOP) top_flush(top);
   if constexpr (WPR == 4) {
     if (lane == 0) joined[wave] = st;
     if constexpr (TOP) {
-      wave_fence();
-      top.buf[lane] = top.best;
+      if (a.splits > 1) {
+        if (lane < a.k)
+          a.pkeys[((row * a.splits + split) * 4 + wave) * a.k + lane] = top.best;
+      } else {
+        keys[wave * 64 + lane] = top.best;
+      }
     }
     __syncthreads();
     if (wave != 0) return;
     st = stat_join(stat_join(joined[0], joined[1]), stat_join(joined[2], joined[3]));
-    if constexpr (TOP) {
-#pragma unroll 1
-      for (int o = 1; o < 4; ++o) {
-        const u64 b = lds[o * 128 + lane];
-        const u64 in = __ballot(b > top.least);  // sorted: the first lanes
-        if (in) top_merge(top, b, __popcll(in));
-      }
-    }
     if (a.splits > 1) {
-      const long long p = row * a.splits + split;
       if (lane == 0) {
-        a.pstat[p * 4] = st.m;
-        a.pstat[p * 4 + 1] = st.s;
-        a.pstat[p * 4 + 2] = st.q;
+        float* p = a.pstat + (row * a.splits + split) * 4;
+        p[0] = st.m;
+        p[1] = st.s;
+        p[2] = st.q;
       }
-      if (TOP && lane < a.k) a.pkeys[p * a.k + lane] = top.best;
       return;
+    }
+    if constexpr (TOP) {
+      // the least of the four lists' ceil(k / 4)-th keys has k keys at or above it
+      const int j = (a.k + 3) / 4 - 1;
+      u64 t = keys[j];
+#pragma unroll
+      for (int o = 1; o < 4; ++o) t = keys[o * 64 + j] < t ? keys[o * 64 + j] : t;
+      if (t > 0) top_raise(top, t - 1);
+#pragma unroll 1
+      for (int o = 1; o < 4; ++o) top_push(top, keys[o * 64 + lane]);
+      top_flush(top);
     }
   }
   float ls = 0.f;
@@ -299,35 +355,78 @@ __global__ __launch_bounds__(kNT) void lp_fwd_kernel(LpArgs a) {
   if constexpr (TOP) top_write(a, row, top.best, __shfl(st.m, 0, 64), __shfl(ls, 0, 64));
 }
 
-// Joins the splits of a row: statistics in one wave, keys in 16 waves of up to
-// four lists each and then in one.
+// Joins the splits of a row: statistics in one wave; keys of up to 256 lists.
+constexpr int kJoinNT = 1024;
 template <int DT, bool TOP>
-__global__ __launch_bounds__(TOP ? 1024 : 64) void lp_join_kernel(LpArgs a) {
-  __shared__ u64 lds[TOP ? 16 * 128 : 1];
-  const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63;
+__global__ __launch_bounds__(TOP ? kJoinNT : 64) void lp_join_kernel(LpArgs a) {
+  constexpr int MAXC = kMaxTop * kMaxTop;  // keys that can be at or above the threshold
+  __shared__ __attribute__((aligned(16))) u64 lds[TOP ? 128 : 1];
+  __shared__ u64 cand[TOP ? MAXC : 1];
+  __shared__ u64 bound;
+  __shared__ int count;
+  const int lane = threadIdx.x & 63;
   const long long row = a.row0 + blockIdx.x;
-  Top top{0, 0, 0, a.k, lds + (TOP ? wave * 128 : 0), lds + (TOP ? wave * 128 + 64 : 0)};
+  const int lists = a.splits * 4;
   if constexpr (TOP) {
-    u64 b[4];
+    // this thread's share of the keys: in flight while the threshold is searched
+    const u64* src = a.pkeys + row * lists * a.k;
+    const int total = lists * a.k;
+    u64 mine[kMaxSplits * 4 * kMaxTop / kJoinNT];
+    constexpr int MINE = sizeof(mine) / 8;
 #pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      const int sp = wave + 16 * i;
-      b[i] = sp < a.splits && lane < a.k ? a.pkeys[(row * a.splits + sp) * a.k + lane] : 0;
+    for (int i = 0; i < MINE; ++i) {
+      const int at = i * kJoinNT + (int)threadIdx.x;
+      mine[i] = at < total ? src[at] : 0;
     }
+    if (threadIdx.x < 64) {
+      const int j = (a.k + lists - 1) / lists, need = (a.k + j - 1) / j;
+      u64 head[4];
 #pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      const u64 in = __ballot(b[i] > top.least);
-      if (in) top_merge(top, b[i], __popcll(in));
+      for (int i = 0; i < 4; ++i) {
+        const int l = i * 64 + lane;
+        head[i] = l < lists ? src[l * a.k + j - 1] : 0;
+      }
+      // the need-th largest: by value, and where equal values leave more, by place
+      uint32_t hi = 0;
+      int n = 0, above = 0;
+      for (uint32_t bit = 0x80000000u; bit; bit >>= 1) {
+        n = 0;
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+          n += __popcll(__ballot((uint32_t)(head[i] >> 32) >= (hi | bit)));
+        if (n >= need) hi |= bit, above = n;
+      }
+      u64 t = (u64)hi << 32;
+      if (hi != 0 && above > need) {
+        for (uint32_t bit = 0x80000000u; bit; bit >>= 1) {
+          n = 0;
+#pragma unroll
+          for (int i = 0; i < 4; ++i) n += __popcll(__ballot(head[i] >= (t | bit)));
+          if (n >= need) t |= bit;
+        }
+      }
+      if (lane == 0) {
+        bound = t;  // 0: lists that are not full
+        count = 0;
+      }
     }
-    top.buf[lane] = top.best;
     __syncthreads();
-    if (wave != 0) return;
-#pragma unroll 1
-    for (int o = 1; o < 16; ++o) {
-      const u64 c = lds[o * 128 + lane];
-      const u64 in = __ballot(c > top.least);
-      if (in) top_merge(top, c, __popcll(in));
+    const u64 t = bound > 0 ? bound : 1;
+#pragma unroll
+    for (int i = 0; i < MINE; ++i) {
+      if (mine[i] >= t) {
+        const int at = atomicAdd(&count, 1);  // any order: the merge sorts
+        if (at < MAXC) cand[at] = mine[i];
+      }
     }
+    __syncthreads();
+    if (threadIdx.x >= 64) return;
+  }
+  Top top = top_new(a.k, lds);
+  if constexpr (TOP) {
+    const int n = min(count, MAXC);
+    for (int i = 0; i < n; i += 64) top_push(top, i + lane < n ? cand[i + lane] : 0);
+    top_flush(top);
   }
   Stat st{-INFINITY, 0.f, 0.f};
   if (lane < a.splits) {
@@ -405,7 +504,8 @@ int lp_fwd(LpArgs a, hipStream_t st) {
       hipLaunchKernelGGL((lp_fwd_kernel<DT, TOP, 4>), dim3((unsigned)(n * a.splits)), dim3(kNT), 0,
                          st, a);
       if (a.splits > 1)
-        hipLaunchKernelGGL((lp_join_kernel<DT, TOP>), dim3((unsigned)n), dim3(TOP ? 1024 : 64), 0,
+        hipLaunchKernelGGL((lp_join_kernel<DT, TOP>), dim3((unsigned)n), dim3(TOP ? kJoinNT : 64),
+                           0,
                            st, a);
     }
     ZK_CHECK_LAUNCH();
@@ -436,7 +536,7 @@ int lp_bwd(LpArgs a, hipStream_t st) {
 ZK_EXPORT long long zk_token_logprobs_ws_bytes(long long rows, int V, int k) {
   if (rows < 1 || V < 1 || k < 0 || k > kMaxTop) return 0;
   const long long s = fwd_splits(rows, V);
-  return s > 1 ? rows * s * (16 + 8LL * k) : 0;
+  return s > 1 ? rows * s * (16 + 4 * 8LL * k) : 0;
 }
 
 // x [rows][xs] logits, tokens [rows] int64 -> logp, entropy [rows] fp32; with
@@ -463,7 +563,7 @@ ZK_EXPORT int zk_token_logprobs_fwd(const void* x, const void* tokens, void* log
   a.top_logp = (float*)top_logp;
   a.top_ids = (long long*)top_ids;
   a.pkeys = (u64*)ws;  // keys first: 8-byte aligned
-  a.pstat = (float*)((char*)ws + rows * splits * 8LL * k);
+  a.pstat = (float*)((char*)ws + rows * splits * 4 * 8LL * k);
   a.rows = rows;
   a.xs = xs;
   a.ignore = ignore;
