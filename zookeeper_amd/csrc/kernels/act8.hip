@@ -439,19 +439,21 @@ __global__ __launch_bounds__(kNT, 2) void dense8_wgrad_kernel(D8Args a) {
 
 // ---------------------------------------------------------------------------
 // The same product for large sizes: a block of 8 waves owns a 256 x 256 tile and
-// walks 64 rows a step in two halves of 32.  dy rows go to LDS by LDS-DMA, one
-// step ahead; codes go through registers, two steps ahead of their use, are
-// decoded between the matrix instructions of the step before and stored as bf16
-// rows.  Two buffers of 64 KB.  One wave holds 128 x 64 of the tile, 32
-// accumulators of 16 x 16.
+// walks 64 rows a step in two halves of 32.  dy rows go to LDS by LDS-DMA, two
+// steps ahead into three buffers; codes go through registers, are decoded between
+// the matrix instructions of the step before their use and stored as bf16 rows into
+// two buffers.  One wave holds 128 x 64 of the tile, 32 accumulators of 16 x 16.
 //
-// Per step and half: the fragments of the other row half of dy are read while
-// this half's products run; every barrier is preceded by the LDS waits of the
-// wave's own reads and writes.  Loads return in order, so a code whose value has
-// arrived proves that the dy pieces asked for before it have landed too; the
-// explicit vmcnt waits count the instructions behind the piece that is needed (2
-// per dy piece, 4 per code piece).  Behind the last row both kinds read valid
-// stand-ins, so the counts never change.
+// One barrier per step, before its last quarter of products: behind it the first
+// fragments of the next step are read while those products run, and nothing reads
+// this step's buffers any more.  (With two dy buffers and two barriers a step took
+// 4800 cycles whatever the load; the products are 2048 and the transposed LDS
+// reads, at the measured 133 B per cycle, 1500.)  Each quarter's fragments are read a
+// quarter ahead, six to eight at a time.  The barrier waits for the wave's own LDS
+// reads and writes.  Loads return in order: the explicit vmcnt wait counts the
+// instructions behind the dy rows that are needed (4 and 4 for the next codes, 4 for
+// the dy rows after them).  Behind the last row both kinds read valid stand-ins, so
+// the counts never change.
 //
 // The rows of a term are padded to whole steps (Mp = M rounded up to 64): dy rows
 // behind M are zeros, so the kept rows beside them may be any that exist.  (A NaN
@@ -465,8 +467,10 @@ __global__ __launch_bounds__(kNT, 2) void dense8_wgrad_kernel(D8Args a) {
 // ---------------------------------------------------------------------------
 constexpr int kW = 256;                 // tile edge
 constexpr int kWNT = 512;               // threads
-constexpr int kWPiece = 32 * kW * 2;    // 32 rows of 512 B
-constexpr int kWBuf = 4 * kWPiece;      // dy halves 0 and 1, x halves 0 and 1
+constexpr int kWPiece = 32 * kW * 2;    // a half: 32 rows of 512 B
+constexpr int kWBuf = 2 * kWPiece;      // a step's dy or x
+constexpr int kWX = 3 * kWBuf;          // x behind three dy buffers
+constexpr int kWLds = 5 * kWBuf;        // all 160 KB of a CU
 
 __device__ __attribute__((aligned(512))) uint4 g_a8_zero[32];  // 512 B of zeros
 
@@ -526,8 +530,8 @@ __global__ __launch_bounds__(kWNT, 2) void dense8_wide_kernel(D8WideArgs a) {
   const unsigned char* dyb = reinterpret_cast<const unsigned char*>(a.dy) + n0 * 2LL;
   const long long dyrow = a.dys * 2;
   const uint32_t aoff = (uint32_t)(arow * (int)dyrow + acol);
-  auto issue = [&](int s, int h) {
-    const uint32_t dst = (s & 1) * kWBuf + h * kWPiece + wave * 1024;
+  auto issue = [&](int s, int h, uint32_t buf) {
+    const uint32_t dst = buf + h * kWPiece + wave * 1024;
     const int rb = r0 + s * 64 + h * 32;  // uniform
     if (rb + 32 <= a.dyrows) {
       const unsigned char* base = dyb + rb * dyrow;
@@ -575,7 +579,7 @@ __global__ __launch_bounds__(kWNT, 2) void dense8_wide_kernel(D8WideArgs a) {
   // the other 16 rows of a half have the same swizzle
   const uint32_t xput = crow * 512 + (((tid & 31) ^ tr_swz<512>(crow)) << 4);
   auto put = [&](const Codes& c, int s, int h) {
-    const uint32_t at = xput | ((s & 1) * kWBuf);
+    const uint32_t at = xput + kWX + (s & 1) * kWBuf;
 #pragma unroll
     for (int i = 0; i < 2; ++i) {
       // E = 255: the step is infinite and 0 codes become inf - inf = NaN
@@ -598,7 +602,7 @@ __global__ __launch_bounds__(kWNT, 2) void dense8_wide_kernel(D8WideArgs a) {
         const float y = (float)((w >> (16 * (j & 1) + 8)) & 0xffu);
         o[j] = bf16_pair(__builtin_fmaf(x, st, off), __builtin_fmaf(y, st, off));
       }
-      *(lds_u128*)(uintptr_t)(at + (2 + h) * kWPiece + i * 8192) = o;
+      *(lds_u128*)(uintptr_t)(at + h * kWPiece + i * 8192) = o;
     }
   };
 
@@ -625,17 +629,17 @@ __global__ __launch_bounds__(kWNT, 2) void dense8_wide_kernel(D8WideArgs a) {
     const s16x8 v = {lo[0], lo[1], lo[2], lo[3], hi[0], hi[1], hi[2], hi[3]};
     return __builtin_bit_cast(uint4, v);
   };
-  auto readD = [&](uint4 (&d)[4], int s, int h, int mh) {
-    uint32_t l = fd | ((s & 1) * kWBuf);
+  auto readD = [&](uint4 (&d)[4], uint32_t buf, int h, int mh) {
+    uint32_t l = fd + buf;
     asm volatile("" : "+v"(l));
 #pragma unroll
     for (int i = 0; i < 4; ++i) d[i] = frag(l, mh * 128 + i * 32, h * kWPiece);
   };
-  auto readX = [&](uint4 (&d)[4], int s, int h) {
-    uint32_t l = fx | ((s & 1) * kWBuf);
+  auto readX = [&](uint4& d0, uint4& d1, int s, int h, int j) {  // fragments j and j + 1
+    uint32_t l = fx + kWX + (s & 1) * kWBuf;
     asm volatile("" : "+v"(l));
-#pragma unroll
-    for (int j = 0; j < 4; ++j) d[j] = frag(l, j * 32, (2 + h) * kWPiece);
+    d0 = frag(l, j * 32, h * kWPiece);
+    d1 = frag(l, j * 32 + 32, h * kWPiece);
   };
   auto mma = [&](const uint4 (&d)[4], const uint4 (&x)[4], int mh) {
 #pragma unroll
@@ -656,56 +660,65 @@ __global__ __launch_bounds__(kWNT, 2) void dense8_wide_kernel(D8WideArgs a) {
   };
 
   Codes c0, c1;
-  issue(0, 0);
+  uint32_t cur = 0, nxt = kWBuf, far = 2 * kWBuf;  // dy buffers of steps s, s + 1, s + 2
+  issue(0, 0, cur);
+  issue(0, 1, cur);
   fetch(c0, 0, 0);
   fetch(c1, 0, 1);
   put(c0, 0, 0);
   put(c1, 0, 1);
   fetch(c0, 1, 0);
-  issue(0, 1);
   fetch(c1, 1, 1);
-  wait_vmcnt<0>();
+  issue(1, 0, nxt);
+  issue(1, 1, nxt);
+  wait_vmcnt<12>();  // dy of step 0
   lds_barrier();
-  readD(d1, 0, 0, 0);
-  readX(x1, 0, 0);
+  readD(d1, cur, 0, 0);
+  readX(x1[0], x1[1], 0, 0, 0);
+  readX(x1[2], x1[3], 0, 0, 2);
   for (int s = 0; s < steps; ++s) {
     const bool sum = a.db && s % a.ktiles == kt;  // uniform
-    // half 0, rows of dy's first columns
-    readD(d2, s, 0, 1);
+    // half 0, the first 64 of the wave's dy columns
+    readD(d2, cur, 0, 1);
+    readX(x2[0], x2[1], s, 1, 0);
     __builtin_amdgcn_sched_barrier(0);
     put(c0, s + 1, 0);
     mma(d1, x1, 0);
     __builtin_amdgcn_sched_barrier(0);
     if (sum) sums(d1, 0);
-    issue(s + 1, 0);
     fetch(c0, s + 2, 0);
     __builtin_amdgcn_sched_barrier(0);
-    wait_vmcnt<10>();  // dy half 1 of this step; behind it: codes, dy, codes
-    lds_barrier();
-    readD(d1, s, 1, 0);
-    readX(x2, s, 1);
+    // ... the second
+    readD(d1, cur, 1, 0);
+    readX(x2[2], x2[3], s, 1, 2);
     __builtin_amdgcn_sched_barrier(0);
     mma(d2, x1, 1);
     if (sum) sums(d2, 1);
     __builtin_amdgcn_sched_barrier(0);
     // half 1
-    readD(d2, s, 1, 1);
+    readD(d2, cur, 1, 1);
     __builtin_amdgcn_sched_barrier(0);
     put(c1, s + 1, 1);
     mma(d1, x2, 0);
     __builtin_amdgcn_sched_barrier(0);
     if (sum) sums(d1, 0);
-    issue(s + 1, 1);
     fetch(c1, s + 2, 1);
+    issue(s + 2, 0, far);
+    issue(s + 2, 1, far);
     __builtin_amdgcn_sched_barrier(0);
-    wait_vmcnt<10>();  // dy half 0 of the next step
+    wait_vmcnt<12>();  // dy of the next step
     lds_barrier();
-    readD(d1, s + 1, 0, 0);
-    readX(x1, s + 1, 0);
+    readD(d1, nxt, 0, 0);
+    readX(x1[0], x1[1], s + 1, 0, 0);
+    readX(x1[2], x1[3], s + 1, 0, 2);
     __builtin_amdgcn_sched_barrier(0);
     mma(d2, x2, 1);
     if (sum) sums(d2, 1);
     __builtin_amdgcn_sched_barrier(0);
+    const uint32_t old = cur;
+    cur = nxt;
+    nxt = far;
+    far = old;
   }
   wait_vmcnt<0>();  // no LDS-DMA may outlive the block
 
@@ -851,9 +864,6 @@ D8Plan dense8_plan(long long M, int N, int K, int dt, long long dys, bool aligne
         s = c;
       }
     }
-#ifdef FS
-    s = FS;
-#endif
     p.rps = ((R + s - 1) / s + 63) / 64 * 64;
     p.splits = (int)((R + p.rps - 1) / p.rps);
   } else {
@@ -885,16 +895,16 @@ int dense8_wide_launch(const D8WideArgs& a, hipStream_t st) {
   if (!g_wide_attr) {
     for (const void* f : {(const void*)dense8_wide_kernel<false>, (const void*)dense8_wide_kernel<true>}) {
       const hipError_t e =
-          hipFuncSetAttribute(f, hipFuncAttributeMaxDynamicSharedMemorySize, 2 * kWBuf);
+          hipFuncSetAttribute(f, hipFuncAttributeMaxDynamicSharedMemorySize, kWLds);
       if (e != hipSuccess) return (int)e;
     }
     g_wide_attr = true;
   }
   const dim3 g((unsigned)(a.ntiles * a.ktiles * a.splits));
   if (a.K & 7)
-    hipLaunchKernelGGL(dense8_wide_kernel<true>, g, dim3(kWNT), 2 * kWBuf, st, a);
+    hipLaunchKernelGGL(dense8_wide_kernel<true>, g, dim3(kWNT), kWLds, st, a);
   else
-    hipLaunchKernelGGL(dense8_wide_kernel<false>, g, dim3(kWNT), 2 * kWBuf, st, a);
+    hipLaunchKernelGGL(dense8_wide_kernel<false>, g, dim3(kWNT), kWLds, st, a);
   return (int)hipGetLastError();
 }
 
