@@ -554,6 +554,7 @@ __global__ __launch_bounds__(kWNT, 2) void dense8_wide_kernel(D8WideArgs a) {
   const int cc = col >= a.K ? 0 : KCUT ? min(col, a.K - 8) : col;
   const int back = col >= a.K ? 0 : 8 * (col - cc);
   const int sc = (col >= a.K ? 0 : col) >> 5;
+  const uint32_t coff = (uint32_t)(crow * a.K + cc), eoff = (uint32_t)(crow * a.kb + sc);
   struct Codes {
     Bytes8 w[2];
     uint32_t e[2];
@@ -564,17 +565,20 @@ __global__ __launch_bounds__(kWNT, 2) void dense8_wide_kernel(D8WideArgs a) {
     for (int i = 0; i < 3; ++i) mb = mb >= a.Mp ? mb - a.Mp : mb;  // past the last: any row
     mb = mb >= a.Mp ? 0 : mb;
     const int m0 = min(mb, a.M - 1);
-    int ra = crow, rb = crow + 16;
-    if (mb + 32 > a.M) {  // rows behind M: the last one
-      ra = min(ra, a.M - 1 - m0);
-      rb = min(rb, a.M - 1 - m0);
-    }
     const int8_t* p = a.codes + (long long)m0 * a.K;
     const uint8_t* q = a.scales + (long long)m0 * a.kb;
-    c.w[0] = *reinterpret_cast<const Bytes8*>(p + (uint32_t)(ra * a.K + cc));
-    c.e[0] = q[(uint32_t)(ra * a.kb + sc)];
-    c.w[1] = *reinterpret_cast<const Bytes8*>(p + (uint32_t)(rb * a.K + cc));
-    c.e[1] = q[(uint32_t)(rb * a.kb + sc)];
+    uint32_t oa = coff, ob = coff + 16 * a.K, ea = eoff, eb = eoff + 16 * a.kb;
+    if (mb + 32 > a.M) {  // uniform; rows behind M: the last one
+      const int ra = min(crow, a.M - 1 - m0), rb = min(crow + 16, a.M - 1 - m0);
+      oa = (uint32_t)(ra * a.K + cc);
+      ob = (uint32_t)(rb * a.K + cc);
+      ea = (uint32_t)(ra * a.kb + sc);
+      eb = (uint32_t)(rb * a.kb + sc);
+    }
+    c.w[0] = *reinterpret_cast<const Bytes8*>(p + oa);
+    c.e[0] = q[ea];
+    c.w[1] = *reinterpret_cast<const Bytes8*>(p + ob);
+    c.e[1] = q[eb];
   };
   // the other 16 rows of a half have the same swizzle
   const uint32_t xput = crow * 512 + (((tid & 31) ^ tr_swz<512>(crow)) << 4);
@@ -838,9 +842,12 @@ struct D8Plan {
 
 D8Plan dense8_plan(long long M, int N, int K, int dt, long long dys, bool aligned, int variant) {
   D8Plan p{};
-  // Measured per call, bf16: 2048 x 256 x 256 19 us (128) / 33 us (256), 4096 x 768 x 768
-  // 60 / 53, 16384 x 1024 x 1024 123 / 92, 16384 x 4096 x 4096 1534 / 641.
-  p.wide = variant == 1 || (variant < 0 && M >= 64 && N >= 128 && K >= 128 &&
+  // us per call, 128 / 256 kernel (rows x outputs x inputs, bf16): 1024 x 1024 x 1024
+  // 27 / 42, 4096 x 512 x 512 31 / 33, 16384 x 1024 x 128 33 / 37, 32768 x 256 x 512
+  // 44 / 44, 512 x 2048 x 2048 35 / 29, 4096 x 768 x 768 58 / 38, 16384 x 1024 x 1024
+  // 99 / 64, 16384 x 4096 x 4096 1437 / 535.
+  p.wide = variant == 1 || (variant < 0 && M >= 64 && N >= 192 && K >= 192 &&
+                            (long long)N * K >= (1 << 18) &&
                             (double)M * N * K >= 2147483648.0);
   const int T = p.wide ? kW : kT;
   p.ntiles = (N + T - 1) / T;
