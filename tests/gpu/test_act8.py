@@ -246,6 +246,33 @@ def test_dense_gradients_of_each_kernel(rows, outs, cols, dt, variant):
     assert torch.equal(w2, dw + 1) and torch.equal(b2, db + 2)
 
 
+@pytest.mark.parametrize("variant", [0, 1])
+def test_dense_gradients_of_extreme_values(variant):
+    """Kept values from the smallest step to the largest, dy scaled against them."""
+    from zookeeper_amd.ops import pack8
+    from zookeeper_amd.ops.act8 import _dense_grads
+
+    torch.manual_seed(7)
+    rows, outs, cols = 130, 70, 128
+    big = torch.finfo(torch.float32).max
+    x = torch.rand(rows, cols, device="cuda") * 2 - 1
+    x[:, :32] *= big
+    x[::3, 0], x[1::3, 1] = big, -big
+    x[:, 32:64] *= 2.0 ** -119
+    x[:, 64:96] *= 2.0 ** -127  # subnormal
+    kept = pack8(x)
+    assert int(kept.scales.max()) == 254 and int(kept.scales.min()) == 7
+    h = _held(x)
+    for scale, lo, hi in ((2.0 ** -40, 0, 32), (2.0 ** 40, 32, 96), (1.0, 96, 128)):
+        dy = torch.randn(rows, outs, device="cuda") * scale
+        for dt in (torch.float32, torch.bfloat16):
+            d = dy.to(dt).double()
+            dw, _ = _dense_grads(dy.to(dt), kept.codes, kept.scales, True, variant=variant)
+            mag = d.abs().t() @ h.abs()
+            err = (dw.double() - d.t() @ h).abs()[:, lo:hi]
+            assert (err <= (rows + 16) * 2.0 ** -23 * mag[:, lo:hi]).all()
+
+
 def test_dense_rows_with_gaps_and_special_values():
     from zookeeper_amd.ops import dense8_grads, pack8
 

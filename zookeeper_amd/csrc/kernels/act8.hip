@@ -39,33 +39,36 @@ __device__ __forceinline__ float step_of(uint32_t E) {  // 2^(E - 133); E = 255:
 
 // The quad's block of 32: scale byte and this lane's 8 codes.
 __device__ __forceinline__ uint32_t encode8(const float (&x)[8], uint32_t (&code)[2]) {
-  uint32_t top = 0;
+  float t = fabsf(x[0]);
 #pragma unroll
-  for (int i = 0; i < 8; ++i) {
-    const uint32_t b = __float_as_uint(x[i]) & 0x7fffffffu;  // NaN > inf > numbers
-    top = b > top ? b : top;
-  }
-  top = quad_max(top);
+  for (int i = 1; i < 8; ++i) t = __builtin_elementwise_maximum(t, fabsf(x[i]));  // keeps a NaN
+  const uint32_t top = quad_max(__float_as_uint(t) & 0x7fffffffu);  // NaN > inf > numbers
   uint32_t E = top >> 23;
   if (E == 255u) {
     code[0] = code[1] = 0u;
     return 255u;
   }
   E = E < 7u ? 7u : E;
-  // 1 / step = 2^(133 - E); both this product and the codes' are exact
+  // 1 / step = 2^(133 - E): products with it are exact
   if (__builtin_rintf(__uint_as_float(top) * __uint_as_float((260u - E) << 23)) >= 128.f && E < 254u)
     ++E;
   const float inv = __uint_as_float((260u - E) << 23);
   uint32_t c[8];
+  // adding 1.5 * 2^23 rounds to a whole number (ties to even) whose two's complement
+  // is in the low byte; only at E = 254 can it be 128
 #pragma unroll
-  for (int i = 0; i < 8; ++i) {
-    // adding 1.5 * 2^23 rounds to a whole number (ties to even) whose two's
-    // complement is in the low byte
-    const float v = __builtin_amdgcn_fmed3f(x[i] * inv, -127.f, 127.f) + 12582912.f;
-    c[i] = __float_as_uint(v) & 0xffu;
+  for (int i = 0; i < 8; ++i) c[i] = __float_as_uint(__builtin_fmaf(x[i], inv, 12582912.f));
+  if (E == 254u) {
+#pragma unroll
+    for (int i = 0; i < 8; ++i)
+      c[i] = __float_as_uint(__builtin_amdgcn_fmed3f(x[i] * inv, -127.f, 127.f) + 12582912.f);
   }
-  code[0] = c[0] | (c[1] << 8) | (c[2] << 16) | (c[3] << 24);
-  code[1] = c[4] | (c[5] << 8) | (c[6] << 16) | (c[7] << 24);
+#pragma unroll
+  for (int i = 0; i < 2; ++i) {  // low bytes of four words: v_perm_b32
+    const uint32_t lo = __builtin_amdgcn_perm(c[4 * i + 1], c[4 * i], 0x0c0c0400u);
+    const uint32_t hi = __builtin_amdgcn_perm(c[4 * i + 3], c[4 * i + 2], 0x04000c0cu);
+    code[i] = lo | hi;
+  }
   return E;
 }
 
@@ -84,7 +87,7 @@ __device__ __forceinline__ void decode8(const uint32_t (&code)[2], uint32_t E, f
 // an even relative error: 1e-7).  The exponential is the normal density's too.
 __device__ __forceinline__ void normal_of(float x, float& cdf, float& e) {
   const float t = __builtin_amdgcn_rcpf(__builtin_fmaf(0.305f, fabsf(x), 1.f));
-  e = __builtin_amdgcn_exp2f(x * x * -0.72134752044448170368f);
+  e = __builtin_amdgcn_exp2f(x * (x * -0.72134752044448170368f));
   float p = 0.036698496726864566f;
   p = __builtin_fmaf(p, t, -0.1529855293523711f);
   p = __builtin_fmaf(p, t, 0.18571227887536676f);
@@ -583,30 +586,39 @@ __global__ __launch_bounds__(kWNT, 2) void dense8_wide_kernel(D8WideArgs a) {
   // the other 16 rows of a half have the same swizzle
   const uint32_t xput = crow * 512 + (((tid & 31) ^ tr_swz<512>(crow)) << 4);
   auto put = [&](const Codes& c, int s, int h) {
-    const uint32_t at = xput + kWX + (s & 1) * kWBuf;
+    const uint32_t at = xput + kWX + (s & 1) * kWBuf + h * kWPiece;
+    const bool far_end = __any(max(c.e[0], c.e[1]) >= 254u);  // NaN blocks, largest steps
 #pragma unroll
     for (int i = 0; i < 2; ++i) {
-      // E = 255: the step is infinite and 0 codes become inf - inf = NaN
-      const uint32_t e = c.e[i];
-      const float st = __uint_as_float((e == 255u ? 255u : e - 6u) << 23);
-      const float off = -128.f * st;
-      uint32_t b0 = c.w[i][0], b1 = c.w[i][1];
+      uint32_t b[2] = {c.w[i][0], c.w[i][1]};
       if constexpr (KCUT) {
-        const u64_t v = (((u64_t)b1 << 32) | b0) >> back;
-        b0 = (uint32_t)v;
-        b1 = (uint32_t)(v >> 32);
+        const u64_t v = (((u64_t)b[1] << 32) | b[0]) >> back;
+        b[0] = (uint32_t)v;
+        b[1] = (uint32_t)(v >> 32);
       }
-      // code + 128 as an unsigned byte: the conversion picks the byte itself
-      const uint32_t b[2] = {b0 ^ 0x80808080u, b1 ^ 0x80808080u};
       u32x4 o;
+      if (far_end) {
+        const float st = step_of(c.e[i]);
 #pragma unroll
-      for (int j = 0; j < 4; ++j) {
-        const uint32_t w = b[j >> 1];
-        const float x = (float)((w >> (16 * (j & 1))) & 0xffu);
-        const float y = (float)((w >> (16 * (j & 1) + 8)) & 0xffu);
-        o[j] = bf16_pair(__builtin_fmaf(x, st, off), __builtin_fmaf(y, st, off));
+        for (int j = 0; j < 4; ++j)
+          o[j] = bf16_pair(code_at(b[j >> 1], 2 * (j & 1)) * st,
+                           code_at(b[j >> 1], 2 * (j & 1) + 1) * st);
+      } else {
+        // code + 128 as an unsigned byte, which the conversion picks itself, and one
+        // fma (538 us at 16384 x 4096 x 4096; signed bytes, v_cvt_f32_i32 with a byte
+        // operand, 570).  At E = 254 the 128 steps to take off would overflow.
+        const float st = __uint_as_float((c.e[i] - 6u) << 23), off = -128.f * st;
+        b[0] ^= 0x80808080u;
+        b[1] ^= 0x80808080u;
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+          const uint32_t w = b[j >> 1];
+          const float x = (float)((w >> (16 * (j & 1))) & 0xffu);
+          const float y = (float)((w >> (16 * (j & 1) + 8)) & 0xffu);
+          o[j] = bf16_pair(__builtin_fmaf(x, st, off), __builtin_fmaf(y, st, off));
+        }
       }
-      *(lds_u128*)(uintptr_t)(at + h * kWPiece + i * 8192) = o;
+      *(lds_u128*)(uintptr_t)(at + i * 8192) = o;
     }
   };
 
