@@ -1,0 +1,174 @@
+"""The row operators (layer norm, log probabilities, 8-bit kept activations) as a
+program uses them: rows farther apart than 32-bit offsets reach, two streams and
+two threads at a time, a model under the trainer with and without graph replay."""
+
+import threading
+
+import pytest
+import torch
+
+pytestmark = pytest.mark.gpu
+
+
+@pytest.fixture(autouse=True)
+def _gpu():
+    if not torch.cuda.is_available():
+        pytest.skip("needs a GPU")
+    from zookeeper_amd import ops
+
+    assert ops.available(), ops.load_error()
+
+
+def test_rows_far_apart():
+    """Row starts past 2^31 elements."""
+    from zookeeper_amd import ops
+
+    torch.manual_seed(0)
+    step = (1 << 30) + 40
+    base = torch.empty(2 * step + 5000, dtype=torch.bfloat16, device="cuda")
+    far = torch.as_strided(base, (3, 5000), (step, 1))
+    near = torch.randn(3, 5000, device="cuda").bfloat16()
+    far.copy_(near)
+    t = torch.randint(0, 5000, (3,), device="cuda")
+    dy = torch.randn(3, 5000, device="cuda").bfloat16()
+
+    def run(v):
+        v = v.detach().requires_grad_(True)
+        y = ops.layer_norm(v)
+        out = [y, torch.autograd.grad(y, v, dy)[0]]
+        r = ops.token_logprobs(v, t, top=7)
+        out += [*r, torch.autograd.grad(r.logp.sum() + r.entropy.sum(), v)[0]]
+        y = ops.gelu8(v)
+        out += [y, torch.autograd.grad(y, v, dy)[0], ops.unpack8(ops.pack8(v.detach()))]
+        # ... as the incoming gradient
+        n = near.detach().requires_grad_(True)
+        g = torch.as_strided(v.detach(), v.shape, v.stride())
+        out += [torch.autograd.grad(ops.layer_norm(n), n, g)[0],
+                torch.autograd.grad(ops.gelu8(n), n, g)[0],
+                *ops.dense8_grads(g, ops.pack8(dy))]
+        return out
+
+    for a, b in zip(run(far), run(near)):
+        assert torch.equal(a, b)
+
+
+def test_more_than_2_31_elements():
+    from zookeeper_amd import ops
+
+    torch.manual_seed(1)
+    rows, cols = 70000, 32768  # 2.3e9 elements
+    x = torch.zeros(rows, cols, dtype=torch.bfloat16, device="cuda")
+    last = torch.randn(3, cols, device="cuda").bfloat16()
+    x[-3:] = last
+    w = torch.rand(cols, device="cuda")
+    assert torch.equal(ops.layer_norm(x, w)[-3:], ops.layer_norm(last, w))
+    t = torch.full((rows,), cols - 1, device="cuda")
+    r, e = ops.token_logprobs(x, t), ops.token_logprobs(last, t[:3])
+    # few rows are split, so the sums differ in their order: at most 32768 / 256 + 64
+    # roundings of s on either side, 2.3e-5
+    torch.testing.assert_close(r.logp[-3:], e.logp, rtol=0, atol=3e-5)
+    kept, want = ops.pack8(x), ops.pack8(last)
+    assert torch.equal(kept.codes[-3:], want.codes) and torch.equal(kept.scales[-3:], want.scales)
+    del kept
+    assert torch.equal(ops.gelu8(x)[-3:], ops.gelu8(last))
+    assert not ops.gelu8(x)[:-3].any()
+
+
+def _program(x, t, w):
+    from zookeeper_amd import ops
+
+    v = x.detach().requires_grad_(True)
+    wl = w.detach().requires_grad_(True)
+    h = ops.layer_norm(v, wl)
+    z = ops.gelu8(h)
+    r = ops.token_logprobs(z, t, top=9)
+    dv, dw = torch.autograd.grad((r.logp - 0.1 * r.entropy).sum(), [v, wl])
+    return [r.logp.detach(), r.entropy.detach(), r.top_ids, dv, dw,
+            *ops.dense8_grads(dv, ops.pack8(z.detach()))]
+
+
+def _case(seed):
+    g = torch.Generator(device="cuda").manual_seed(seed)
+    x = torch.randn(700, 2500, device="cuda", generator=g)
+    return (x, torch.randint(0, 2500, (700,), device="cuda", generator=g),
+            torch.rand(2500, device="cuda", generator=g))
+
+
+def test_two_streams_at_a_time():
+    cases = [_case(s) for s in range(4)]
+    want = [_program(*c) for c in cases]
+    torch.cuda.synchronize()
+    streams = [torch.cuda.Stream() for _ in range(4)]
+    got = [None] * 4
+    for _ in range(3):
+        for i, s in enumerate(streams):
+            with torch.cuda.stream(s):
+                got[i] = _program(*cases[i])
+    torch.cuda.synchronize()
+    for a, b in zip(got, want):
+        assert all(torch.equal(p, q) for p, q in zip(a, b))
+
+
+def test_two_threads_at_a_time():
+    cases = [_case(s) for s in range(3)]
+    want = [_program(*c) for c in cases]
+    torch.cuda.synchronize()
+    got, bad = [None] * 3, []
+
+    def work(i):
+        try:
+            with torch.cuda.stream(torch.cuda.Stream()):
+                for _ in range(4):
+                    got[i] = _program(*cases[i])
+                torch.cuda.current_stream().synchronize()
+        except Exception as e:  # noqa: BLE001
+            bad.append(e)
+
+    threads = [threading.Thread(target=work, args=(i,)) for i in range(3)]
+    for th in threads:
+        th.start()
+    for th in threads:
+        th.join()
+    assert not bad, bad
+    for a, b in zip(got, want):
+        assert all(torch.equal(p, q) for p, q in zip(a, b))
+
+
+def _trainer(graph):
+    from zookeeper_amd import nn as znn
+    from zookeeper_amd.core import configure
+    from zookeeper_amd.ops import token_logprobs
+    from zookeeper_amd.train import SGD, Trainer
+
+    torch.manual_seed(3)
+    model = torch.nn.Sequential(
+        znn.LayerNorm(48), znn.QuantDense(48, 96, use_bias=True, kept="int8"),
+        znn.GELU(kept="int8"), znn.QuantDense(96, 10, use_bias=True, kept="int8"))
+
+    def loss(logits, labels):
+        r = token_logprobs(logits, labels, top=1)
+        return -(r.logp + 0.01 * r.entropy).mean(), (r.top_ids[:, 0] == labels).sum()
+
+    spec = SGD()
+    configure(spec, {"learning_rate": 0.1, "momentum": 0.9})
+    return Trainer(model, loss, spec, graph=graph, graph_warmup=2)
+
+
+def test_a_model_under_the_trainer():
+    """Gradients go straight into the flat buffer; graph replays follow the eager
+    steps bit for bit."""
+    eager, graph = _trainer(False), _trainer(True)
+    g = torch.Generator(device="cuda").manual_seed(4)
+    losses = []
+    for step in range(7):
+        x = torch.randn(300, 48, device="cuda", generator=g)
+        y = torch.randint(0, 10, (300,), device="cuda", generator=g)
+        a, hits = eager.train_step(x, y)
+        b, ghits = graph.train_step(x, y)
+        torch.cuda.synchronize()
+        assert float(a) == float(b) and int(hits) == int(ghits), step
+        assert torch.equal(eager.flat.grad, graph.flat.grad), step
+        assert torch.equal(eager.flat.data, graph.flat.data), step
+        losses.append(float(a))
+    assert graph._graph is not None
+    assert eager.flat.grad.abs().sum() > 0 and len(set(losses)) == 7

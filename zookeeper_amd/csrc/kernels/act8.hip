@@ -793,54 +793,87 @@ __global__ __launch_bounds__(kNT) void dense8_terms_kernel(const void* dy, long 
   }
 }
 
-// out[i] (+)= sum over p of part[p][i].  Few parts: 4 values per thread, the parts in
-// order.
-__global__ __launch_bounds__(kNT) void dense8_sum4_kernel(const float* __restrict__ part,
-                                                          int parts, long long n,
-                                                          float* __restrict__ out, int add) {
-  const long long i = ((long long)blockIdx.x * kNT + threadIdx.x) * 4;
-  if (i >= n) return;
-  if (i + 4 <= n && (n & 3) == 0) {
-    f32x4 s = *reinterpret_cast<const f32x4*>(part + i);
-    for (int p = 1; p < parts; ++p) s += *reinterpret_cast<const f32x4*>(part + p * n + i);
-    if (add) s += *reinterpret_cast<const f32x4*>(out + i);
-    *reinterpret_cast<f32x4*>(out + i) = s;
+// out[i] (+)= sum over p of part[p][i], in a fixed order, for dW and db in one launch.
+struct D8Sum {
+  const float* part;
+  float* out;
+  long long n;
+  int parts, add;
+  int blocks;  // of this sum
+  bool wide;   // 4 values per thread, the parts in order; else sliced
+};
+constexpr int kSumNT = 1024;
+
+__device__ __forceinline__ void sum_wide(const D8Sum& a, long long block) {
+  typedef float f32x4u __attribute__((ext_vector_type(4), aligned(4)));  // odd sizes
+  const long long i = (block * kSumNT + threadIdx.x) * 4;
+  if (i >= a.n) return;
+  const float* q = a.part + i;
+  if (i + 4 <= a.n) {
+    f32x4 s = *reinterpret_cast<const f32x4u*>(q);
+    int p = 1;
+    for (; p + 4 <= a.parts; p += 4) {  // four loads in flight
+      f32x4 v[4];
+#pragma unroll
+      for (int j = 0; j < 4; ++j) v[j] = *reinterpret_cast<const f32x4u*>(q + (p + j) * a.n);
+#pragma unroll
+      for (int j = 0; j < 4; ++j) s += v[j];
+    }
+    for (; p < a.parts; ++p) s += *reinterpret_cast<const f32x4u*>(q + p * a.n);
+    if (a.add) s += *reinterpret_cast<const f32x4u*>(a.out + i);
+    *reinterpret_cast<f32x4u*>(a.out + i) = s;
   } else {
-    for (long long j = i; j < n && j < i + 4; ++j) {
-      float s = part[j];
-      for (int p = 1; p < parts; ++p) s += part[p * n + j];
-      out[j] = add ? s + out[j] : s;
+    for (long long j = i; j < a.n; ++j) {
+      float s = a.part[j];
+      for (int p = 1; p < a.parts; ++p) s += a.part[p * a.n + j];
+      a.out[j] = a.add ? s + a.out[j] : s;
     }
   }
 }
 
-// Many parts: 16 slices of them side by side, each in order, joined in order.
-__global__ __launch_bounds__(1024) void dense8_sum_kernel(const float* __restrict__ part,
-                                                          int parts, long long n,
-                                                          float* __restrict__ out, int add) {
-  __shared__ float red[16][64];
+// many parts of few values: 16 slices of the parts side by side, each in order, joined
+// in order
+__device__ __forceinline__ void sum_sliced(const D8Sum& a, long long block, float (&red)[16][64]) {
   const int col = threadIdx.x & 63, sl = threadIdx.x >> 6;
-  const long long i = (long long)blockIdx.x * 64 + col;
+  const long long i = block * 64 + col;
   float s = 0.f;
-  if (i < n)
-    for (int p = sl; p < parts; p += 16) s += part[(long long)p * n + i];
+  if (i < a.n) {
+    const float* q = a.part + sl * a.n + i;
+    int p = sl;
+    for (; p + 48 < a.parts; p += 64, q += 64 * a.n) {  // four loads in flight
+      float v[4];
+#pragma unroll
+      for (int j = 0; j < 4; ++j) v[j] = q[16 * j * a.n];
+#pragma unroll
+      for (int j = 0; j < 4; ++j) s += v[j];
+    }
+    for (; p < a.parts; p += 16, q += 16 * a.n) s += *q;
+  }
   red[sl][col] = s;
   __syncthreads();
-  if (sl == 0 && i < n) {
+  if (sl == 0 && i < a.n) {
 #pragma unroll
     for (int o = 1; o < 16; ++o) s += red[o][col];
-    out[i] = add ? out[i] + s : s;
+    a.out[i] = a.add ? a.out[i] + s : s;
   }
 }
 
-int dense8_sum(const float* part, int parts, long long n, float* out, int add, hipStream_t st) {
-  if (parts <= 8 || n >= (1 << 20))
-    hipLaunchKernelGGL(dense8_sum4_kernel, dim3((unsigned)((n + 4 * kNT - 1) / (4 * kNT))),
-                       dim3(kNT), 0, st, part, parts, n, out, add);
-  else
-    hipLaunchKernelGGL(dense8_sum_kernel, dim3((unsigned)((n + 63) / 64)), dim3(1024), 0, st, part,
-                       parts, n, out, add);
-  return (int)hipGetLastError();
+__global__ __launch_bounds__(kSumNT) void dense8_sum_kernel(D8Sum dw, D8Sum db) {
+  __shared__ float red[16][64];
+  const bool first = (int)blockIdx.x < dw.blocks;
+  const D8Sum& a = first ? dw : db;
+  const long long block = first ? blockIdx.x : blockIdx.x - dw.blocks;
+  if (a.wide) {
+    sum_wide(a, block);
+  } else {
+    sum_sliced(a, block, red);
+  }
+}
+
+D8Sum dense8_sum(const float* part, int parts, long long n, float* out, int add) {
+  const bool wide = parts <= 8 || n >= (1 << 18);
+  const long long per = wide ? 4LL * kSumNT : 64;
+  return D8Sum{part, out, n, parts, add, (int)((n + per - 1) / per), wide};
 }
 
 // Sizes and workspace of one call.  wide: the 256 x 256 kernel.
@@ -908,16 +941,18 @@ bool dense8_ok(long long M, int N, int K, long long dys) {
          ((N + kT - 1LL) / kT) * ((K + kT - 1LL) / kT) < (1 << 20);
 }
 
-bool g_wide_attr = false;
-
 int dense8_wide_launch(const D8WideArgs& a, hipStream_t st) {
-  if (!g_wide_attr) {
-    for (const void* f : {(const void*)dense8_wide_kernel<false>, (const void*)dense8_wide_kernel<true>}) {
-      const hipError_t e =
-          hipFuncSetAttribute(f, hipFuncAttributeMaxDynamicSharedMemorySize, kWLds);
+  static bool ready[64];  // by device: over 64 KB of LDS are allowed per kernel and device
+  int dev = 0;
+  hipError_t e = hipGetDevice(&dev);
+  if (e != hipSuccess) return (int)e;
+  if (dev < 0 || dev >= 64 || !ready[dev]) {
+    for (const void* f :
+         {(const void*)dense8_wide_kernel<false>, (const void*)dense8_wide_kernel<true>}) {
+      e = hipFuncSetAttribute(f, hipFuncAttributeMaxDynamicSharedMemorySize, kWLds);
       if (e != hipSuccess) return (int)e;
     }
-    g_wide_attr = true;
+    if (dev >= 0 && dev < 64) ready[dev] = true;
   }
   const dim3 g((unsigned)(a.ntiles * a.ktiles * a.splits));
   if (a.K & 7)
@@ -1011,9 +1046,12 @@ ZK_EXPORT int zk_dense8_wgrad(const void* dy, const void* codes, const void* sca
     if (dt == 2) hipLaunchKernelGGL(dense8_wgrad_kernel<2>, g, dim3(kNT), 0, st, a);
     ZK_CHECK_LAUNCH();
   }
-  if (p.splits > 1) {
-    const int e = dense8_sum(slab, p.splits, (long long)N * K, (float*)dw, add & 1, st);
-    if (e) return e;
-  }
-  return db ? dense8_sum(slab + p.slab, p.splits * p.ktiles, N, (float*)db, (add >> 1) & 1, st) : 0;
+  D8Sum sw{}, sb{};
+  if (p.splits > 1) sw = dense8_sum(slab, p.splits, (long long)N * K, (float*)dw, add & 1);
+  if (db) sb = dense8_sum(slab + p.slab, p.splits * p.ktiles, N, (float*)db, (add >> 1) & 1);
+  if (sw.blocks + sb.blocks > 0)
+    hipLaunchKernelGGL(dense8_sum_kernel, dim3((unsigned)(sw.blocks + sb.blocks)), dim3(kSumNT), 0,
+                       st, sw, sb);
+  ZK_CHECK_LAUNCH();
+  return 0;
 }

@@ -43,7 +43,7 @@ typedef unsigned long long u64;
 
 constexpr int kNT = 256;
 constexpr float kL2E = 1.44269504088896340736f;
-constexpr float kLow = -1e30f;  // stands for -inf where it is multiplied by a 0
+constexpr float kLow = -1e4f;  // for differences where e^d is 0: finite times 0 is 0
 constexpr int kMaxSplits = 64;
 constexpr int kMaxTop = 64;
 

@@ -41,8 +41,7 @@ def use_kernels(t: torch.Tensor, what: str) -> bool:
 
 
 def guard(t: torch.Tensor):
-    """Context that makes ``t``'s device the current one for a launch.  (A backward
-    needs none: autograd runs it on a thread of its tensors' device.)"""
+    """Context that makes ``t``'s device the current one for a launch."""
     if t.device.index == torch._C._cuda_getDevice():
         return _HERE
     return torch.cuda.device(t.device)

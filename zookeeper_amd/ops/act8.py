@@ -189,8 +189,9 @@ class _Gelu8Fn(torch.autograd.Function):
             dx = torch.empty(dy.shape, dtype=dy.dtype, device=dev)
             dy2, _, stride = rows_of(dy)
         codes = kept.data_ptr()
-        call(lib().zk_gelu8_bwd, "zk_gelu8_bwd", dy2.data_ptr(), codes, codes + rows * n,
-             dx.data_ptr(), rows, n, stride, DTYPE_CODES[dy.dtype], raw_stream(dev.index))
+        with guard(dy):
+            call(lib().zk_gelu8_bwd, "zk_gelu8_bwd", dy2.data_ptr(), codes, codes + rows * n,
+                 dx.data_ptr(), rows, n, stride, DTYPE_CODES[dy.dtype], raw_stream(dev.index))
         return dx
 
 

@@ -98,9 +98,10 @@ class _LayerNormFn(torch.autograd.Function):
         if rows:
             mean = stats.data_ptr()
             w = as_fp32(weight)
-            call(L.zk_layer_norm_bwd, "zk_layer_norm_bwd", dy2.data_ptr(), x2.data_ptr(), ptr(w),
-                 mean, mean + 4 * rows, ptr(dx), ptr(dw), ptr(db), ptr(ws), ws_bytes, rows, cols,
-                 stride, dys, DTYPE_CODES[x.dtype], add, raw_stream(dev.index))
+            with guard(x):
+                call(L.zk_layer_norm_bwd, "zk_layer_norm_bwd", dy2.data_ptr(), x2.data_ptr(),
+                     ptr(w), mean, mean + 4 * rows, ptr(dx), ptr(dw), ptr(db), ptr(ws), ws_bytes,
+                     rows, cols, stride, dys, DTYPE_CODES[x.dtype], add, raw_stream(dev.index))
         if dw_direct is not None:
             grad_ready(wp)
             dw = None

@@ -92,10 +92,11 @@ class _TokenLogProbsFn(torch.autograd.Function):
             g_logp = g_logp.contiguous()
         if g_entropy is not None and not g_entropy.is_contiguous():
             g_entropy = g_entropy.contiguous()
-        call(lib().zk_token_logprobs_bwd, "zk_token_logprobs_bwd", x.data_ptr(),
-             tokens.data_ptr(), stats.data_ptr(), ptr(g_logp), ptr(g_entropy), dx.data_ptr(),
-             rows, logits.shape[-1], stride, ignore, DTYPE_CODES[logits.dtype],
-             raw_stream(logits.device.index))
+        with guard(logits):
+            call(lib().zk_token_logprobs_bwd, "zk_token_logprobs_bwd", x.data_ptr(),
+                 tokens.data_ptr(), stats.data_ptr(), ptr(g_logp), ptr(g_entropy), dx.data_ptr(),
+                 rows, logits.shape[-1], stride, ignore, DTYPE_CODES[logits.dtype],
+                 raw_stream(logits.device.index))
         return dx, None, None, None
 
 
