@@ -13,6 +13,7 @@ from zookeeper_amd.ops import _native
 
 # element type codes of the C ABI (csrc/kernels/rows.h)
 DTYPE_CODES = {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2}
+_FLOATS = (torch.float32, torch.bfloat16, torch.float16, torch.float64)
 
 # Raw hipStream_t of torch's current stream on a device index.
 raw_stream = torch._C._cuda_getCurrentRawStream
@@ -31,6 +32,8 @@ def use_kernels(t: torch.Tensor, what: str) -> bool:
     """True for a GPU tensor (the HIP kernels run; :func:`_native.lib` raises
     if the library is missing), False for the plain PyTorch form: host tensors,
     or the native path switched off with ``ZK_NATIVE=0``."""
+    if t.is_cuda and t.dtype in DTYPE_CODES and _native.available():
+        return True
     if not t.is_cuda or _native.native_disabled():
         if not t.is_floating_point():
             raise ValueError(f"{what}: expected a floating-point tensor, got {t.dtype}")
@@ -62,6 +65,8 @@ def rows_of(t: torch.Tensor) -> Tuple[torch.Tensor, int, int]:
 
 
 def check_param(p, cols: int, x: torch.Tensor, what: str) -> None:
+    if p.shape == (cols,) and p.device == x.device and p.dtype in _FLOATS:
+        return
     if p.dim() != 1 or p.shape[0] != cols:
         raise ValueError(f"{what}: expected shape ({cols},), got {tuple(p.shape)}")
     if p.device != x.device:
