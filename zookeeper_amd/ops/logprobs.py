@@ -11,7 +11,8 @@ Log probability and entropy are differentiable in the logits (policy losses,
 distillation, entropy bonuses); one pass over the logits forward, one backward.
 The alternatives are for reporting and carry no gradient.
 
-* A token equal to ``ignore_index`` (inside ``[0, V)`` or not) gives log probability 0 and no gradient.
+* A token equal to ``ignore_index`` (inside ``[0, V)`` or not) gives log
+  probability 0 without gradient; the row's entropy is not affected.
 * Masked logits are ``-inf``: probability 0, no share in the entropy.  A row of
   nothing but ``-inf`` has log probability ``-inf``, entropy 0, gradient 0.
 * Any other token outside ``[0, V)`` gives NaN, as does a row with a NaN or
