@@ -172,3 +172,24 @@ def test_a_model_under_the_trainer():
         losses.append(float(a))
     assert graph._graph is not None
     assert eager.flat.grad.abs().sum() > 0 and len(set(losses)) == 7
+
+
+def test_saved_tensors_may_change_their_layout():
+    """Hooks that keep saved tensors elsewhere give padded rows back contiguous."""
+    from zookeeper_amd import ops
+
+    torch.manual_seed(5)
+    wide = torch.randn(50, 3000, device="cuda")
+    x = wide[:, 7:907].detach().requires_grad_(True)
+    w = torch.rand(900, device="cuda", requires_grad=True)
+    t = torch.randint(0, 900, (50,), device="cuda")
+
+    def run():
+        r = ops.token_logprobs(x, t)
+        h = ops.gelu8(ops.dense8(ops.layer_norm(x, w), torch.eye(900, device="cuda")))
+        return torch.autograd.grad(r.logp.sum() + r.entropy.sum() + h.sum(), [x, w])
+
+    want = run()
+    with torch.autograd.graph.save_on_cpu():
+        got = run()
+    assert all(torch.equal(a, b) for a, b in zip(got, want))

@@ -30,8 +30,7 @@ def _ws_bytes(rows: int, cols: int) -> int:
 
 
 def _forward(x, weight, bias, eps: float, stats: bool):
-    """``y``, the rows' mean and rstd ([2, rows] fp32, or None), and what the
-    backward's launch repeats: rows, row stride."""
+    """``y`` and the rows' mean and rstd ([2, rows] fp32, or None)."""
     x2, rows, stride = rows_of(x)
     dev = x.device
     y = torch.empty_like(x) if x.is_contiguous() else torch.empty(x.shape, dtype=x.dtype,
@@ -46,18 +45,19 @@ def _forward(x, weight, bias, eps: float, stats: bool):
         call(lib().zk_layer_norm_fwd, "zk_layer_norm_fwd", x2.data_ptr(), ptr(w), ptr(b),
              y.data_ptr(), mean, rstd, rows, x.shape[-1], stride, eps, DTYPE_CODES[x.dtype],
              raw_stream(dev.index))
-    return y, st, rows, stride
+    return y, st
 
 
 class _LayerNormFn(torch.autograd.Function):
     # Small rows wait for this host code and not for the kernels (a backward
-    # runs on a cold thread): everything that the forward knows is passed on.
+    # runs on a cold thread): as few calls as possible.  The row stride is taken
+    # anew: hooks on saved tensors may give ``x`` back in another layout.
     @staticmethod
     def forward(ctx, x, weight, bias, eps):
-        y, stats, rows, stride = _forward(x, weight, bias, eps, True)
+        y, stats = _forward(x, weight, bias, eps, True)
         ctx.save_for_backward(x, weight)
         # the parameters themselves: the flat gradient buffer hangs on them
-        ctx.rest = (stats, rows, stride, weight, bias)
+        ctx.rest = (stats, weight, bias)
         return y
 
     @staticmethod
@@ -65,10 +65,10 @@ class _LayerNormFn(torch.autograd.Function):
         if torch.is_grad_enabled():
             refuse_twice("layer_norm")
         x, weight = ctx.saved_tensors
-        stats, rows, stride, wp, bp = ctx.rest
+        stats, wp, bp = ctx.rest
         need_x, need_w, need_b = ctx.needs_input_grad[:3]
         dev, cols = x.device, x.shape[-1]
-        x2 = x if x.is_contiguous() else rows_of(x)[0]
+        x2, rows, stride = rows_of(x)
         dx = ws = dw = db = dw_direct = db_direct = None
         add = ws_bytes = 0
         if dy.is_contiguous():

@@ -60,16 +60,15 @@ def _forward(logits, tokens, top: int, ignore: int, keep: bool):
              logp.data_ptr(), entropy.data_ptr(), ptr(stats), ptr(top_logp), ptr(top_ids),
              ptr(ws), ws_bytes, rows, V, stride, top, ignore, DTYPE_CODES[logits.dtype],
              raw_stream(dev.index))
-    return logp, entropy, top_logp, top_ids, stats, rows, stride
+    return logp, entropy, top_logp, top_ids, stats
 
 
 class _TokenLogProbsFn(torch.autograd.Function):
     @staticmethod
     def forward(ctx, logits, tokens, top, ignore):
-        (logp, entropy, top_logp, top_ids, stats, rows,
-         stride) = _forward(logits, tokens, top, ignore, True)
+        logp, entropy, top_logp, top_ids, stats = _forward(logits, tokens, top, ignore, True)
         ctx.save_for_backward(logits, tokens)
-        ctx.rest = (stats, rows, stride, ignore)
+        ctx.rest = (stats, ignore)
         ctx.set_materialize_grads(False)
         if top:
             ctx.mark_non_differentiable(top_logp, top_ids)
@@ -83,11 +82,11 @@ class _TokenLogProbsFn(torch.autograd.Function):
         if g_logp is None and g_entropy is None:
             return None, None, None, None
         logits, tokens = ctx.saved_tensors
-        stats, rows, stride, ignore = ctx.rest
+        stats, ignore = ctx.rest
+        x, rows, stride = rows_of(logits)  # anew: hooks on saved tensors may change the layout
         if logits.is_contiguous():
-            x, dx = logits, torch.empty_like(logits)
+            dx = torch.empty_like(logits)
         else:
-            x = rows_of(logits)[0]
             dx = torch.empty(logits.shape, dtype=logits.dtype, device=logits.device)
         if g_logp is not None and not g_logp.is_contiguous():
             g_logp = g_logp.contiguous()
