@@ -193,3 +193,89 @@ def test_saved_tensors_may_change_their_layout():
     with torch.autograd.graph.save_on_cpu():
         got = run()
     assert all(torch.equal(a, b) for a, b in zip(got, want))
+
+
+class _Delay(torch.autograd.Function):
+    """Identity whose backward keeps the stream it runs on busy for a moment."""
+
+    @staticmethod
+    def forward(ctx, x):
+        return x.view_as(x)
+
+    @staticmethod
+    def backward(ctx, g):
+        torch.cuda._sleep(20_000_000)
+        return g
+
+
+def _shared_model():
+    from zookeeper_amd import nn as znn
+    from zookeeper_amd.parallel.flat import FlatParams
+
+    torch.manual_seed(6)
+    model = torch.nn.Sequential(znn.LayerNorm(64),
+                                znn.QuantDense(64, 64, use_bias=True, kept="int8")).cuda()
+    return model, FlatParams(model)
+
+
+@pytest.mark.parametrize("streams", [1, 2])
+def test_layers_applied_twice_with_flat_gradients(streams):
+    """Two branches through the same layers, each on its own stream: their writes
+    into the flat gradients do not overlap, the caller's stream waits for them,
+    and each parameter is reported ready once, with both contributions."""
+    model, flat = _shared_model()
+    xs = [torch.randn(256, 64, device="cuda") for _ in range(2)]
+    flat.zero_grad()
+    (model(xs[0]).square().sum() + model(xs[1]).square().sum()).backward()
+    torch.cuda.synchronize()
+    want = flat.grad.clone()
+    single = []
+    for x in xs:
+        flat.zero_grad()
+        model(x).square().sum().backward()
+        torch.cuda.synchronize()
+        single.append(flat.grad.clone())
+    # each pass's sums are the same bits, and one addition joins them
+    assert torch.equal(want, single[0] + single[1])
+
+    seen = {}
+    for slot in flat.slots:
+        def ready(slot=slot):
+            assert slot.name not in seen
+            seen[slot.name] = slot.param.grad.clone()
+        slot.param._zk_grad_ready = ready
+    main = torch.cuda.current_stream()
+    side = [main] + [torch.cuda.Stream() for _ in range(streams - 1)]
+    for _ in range(3):
+        flat.zero_grad()
+        seen.clear()
+        sums = []
+        for i, x in enumerate(xs):
+            s = side[i % streams]
+            s.wait_stream(main)
+            with torch.cuda.stream(s):
+                sums.append(_Delay.apply(model(x).square()).sum())
+        for s in side[1:]:
+            main.wait_stream(s)
+        (sums[0] + sums[1]).backward()
+        got = flat.grad.clone()  # on the caller's stream, with no other wait
+        torch.cuda.synchronize()
+        assert torch.equal(got, want)
+        assert sorted(seen) == sorted(s.name for s in flat.slots)
+        for slot in flat.slots:
+            assert torch.equal(seen[slot.name], slot.param.grad)
+
+
+def test_a_dropped_graph_does_not_hold_back_a_parameter():
+    model, flat = _shared_model()
+    count = []
+    for slot in flat.slots:
+        slot.param._zk_grad_ready = lambda name=slot.name: count.append(name)
+    x = torch.randn(8, 64, device="cuda")
+    model(x)  # recorded and dropped
+    model(x).sum().backward()
+    assert sorted(count) == sorted(s.name for s in flat.slots)
+    y = model(x).sum()
+    y.backward(retain_graph=True)
+    y.backward()
+    assert len(count) == 3 * len(flat.slots)

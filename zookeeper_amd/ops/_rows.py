@@ -1,11 +1,13 @@
 """What the row operators (layer norm, log probabilities, 8-bit kept
 activations) share: element type codes of the C ABI, the view of a tensor as
-rows, argument checks and the device guard around a launch."""
+rows, argument checks, the device guard around a launch and the writes into
+flat gradient buffers."""
 
 from __future__ import annotations
 
 import contextlib
-from typing import Tuple
+import weakref
+from typing import Dict, Optional, Tuple
 
 import torch
 
@@ -84,6 +86,76 @@ def as_fp32(p):
 
 def ptr(t):
     return None if t is None else t.data_ptr()
+
+
+class _Use:
+    """One recorded use of a parameter whose gradient is still to come."""
+
+    __slots__ = ("__weakref__",)
+
+
+def note_uses(*params):
+    """Forward: a token for each parameter a data-parallel bucketer waits for
+    (None otherwise).  A token lives as long as the recorded graph, so a graph
+    that is dropped without a backward leaves none behind."""
+    tokens = []
+    for p in params:
+        token = None
+        if p is not None and getattr(p, "_zk_grad_ready", None) is not None:
+            token = _Use()
+            p.__dict__.setdefault("_zk_uses", weakref.WeakSet()).add(token)
+        tokens.append(token)
+    return tokens
+
+
+def last_use_ready(p, token) -> None:
+    """Backward: tell the bucketer that ``p``'s gradient is complete, once no
+    other recorded use of ``p`` is to come (a layer applied twice)."""
+    if token is not None:
+        uses = p.__dict__["_zk_uses"]
+        uses.discard(token)
+        if uses:
+            return
+    _native.grad_ready(p)
+
+
+# Streams that added into flat gradients, by backward pass and parameter.
+_WRITERS: Dict[int, Dict[int, Tuple[torch.device, int]]] = {}
+
+
+def _stream(device: torch.device, raw: int):
+    if raw == 0:
+        return torch.cuda.default_stream(device)
+    return torch.cuda.ExternalStream(raw, device)
+
+
+def _join_writers(task: int) -> None:
+    for device, raw in set(_WRITERS.pop(task, {}).values()):
+        if raw != raw_stream(device.index):
+            torch.cuda.current_stream(device).wait_stream(_stream(device, raw))
+
+
+def flat_grad(p) -> Optional[torch.Tensor]:
+    """:func:`_native.direct_grad` for a parameter that may be used on several
+    streams in one backward pass.  Autograd orders the gradients it accumulates
+    and knows nothing of these: each write waits for the one before it on
+    another stream, and the caller's stream for all of them at the pass's end."""
+    g = _native.direct_grad(p)
+    if g is None:
+        return None
+    task = torch._C._current_graph_task_id()
+    if task < 0:  # not inside a backward pass: one stream, the caller's
+        return g
+    writers = _WRITERS.get(task)
+    if writers is None:
+        writers = _WRITERS[task] = {}
+        torch.autograd.Variable._execution_engine.queue_callback(lambda: _join_writers(task))
+    here = (g.device, raw_stream(g.device.index))
+    last = writers.get(id(p), here)
+    writers[id(p)] = here
+    if last != here:
+        torch.cuda.current_stream(g.device).wait_stream(_stream(*last))
+    return g
 
 
 def refuse_twice(what: str) -> None:

@@ -29,9 +29,10 @@ from typing import Optional, Tuple
 import torch
 import torch.nn.functional as F
 
-from zookeeper_amd.ops._native import direct_grad, grad_ready, lib
-from zookeeper_amd.ops._rows import (DTYPE_CODES, call, guard, ptr, raw_stream, refuse_twice,
-                                     rows_of, use_kernels)
+from zookeeper_amd.ops._native import lib
+from zookeeper_amd.ops._rows import (DTYPE_CODES, call, flat_grad, guard, last_use_ready,
+                                     note_uses, ptr, raw_stream, refuse_twice, rows_of,
+                                     use_kernels)
 
 BLOCK = 32
 
@@ -287,6 +288,7 @@ class _Dense8Fn(torch.autograd.Function):
             codes, scales = kept.codes, kept.scales
         ctx.save_for_backward(codes, scales, weight)
         ctx.weight_param, ctx.bias_param = weight, bias
+        ctx.uses = note_uses(weight, bias)
         return y
 
     @staticmethod
@@ -296,11 +298,12 @@ class _Dense8Fn(torch.autograd.Function):
         codes, scales, weight = ctx.saved_tensors
         need_x, need_w, need_b = ctx.needs_input_grad
         wp, bp = ctx.weight_param, ctx.bias_param
+        wuse, buse = ctx.uses
         dx = torch.matmul(dy, weight.to(dy.dtype)) if need_x else None
         dw = db = None
         native = use_kernels(dy, "dense8")
-        dw_direct = direct_grad(wp) if need_w and native else None
-        db_direct = direct_grad(bp) if need_b and native else None
+        dw_direct = flat_grad(wp) if need_w and native else None
+        db_direct = flat_grad(bp) if need_b and native else None
         if need_w and native:
             dw, db = _dense_grads(dy, codes, scales, need_b, dw_direct, db_direct)
         elif need_w:
@@ -310,12 +313,12 @@ class _Dense8Fn(torch.autograd.Function):
             if db_direct is not None:
                 db_direct += db
         if dw_direct is not None:
-            grad_ready(wp)
+            last_use_ready(wp, wuse)
             dw = None
         elif dw is not None:
             dw = dw.to(wp.dtype)
         if db_direct is not None:
-            grad_ready(bp)
+            last_use_ready(bp, buse)
             db = None
         elif db is not None:
             db = db.to(bp.dtype)
