@@ -27,39 +27,39 @@ def listed():
     return [
         # --- layer norm -----------------------------------------------------
         # one token at a time through a wide model: latency
-        dict(name="norm one token", op="norm", rows=1, cols=4096, dtype="bf16", affine=2,
+        dict(name="norm, one token", op="norm", rows=1, cols=4096, dtype="bf16", affine=2,
              train=False),
         # a training step's rows, forward and backward with the weight's gradient
-        dict(name="norm training rows", op="norm", rows=32768, cols=2048, dtype="bf16",
+        dict(name="norm, training rows", op="norm", rows=32768, cols=2048, dtype="bf16",
              affine=2, train=True),
         # odd row count, odd width, full precision
-        dict(name="norm odd width", op="norm", rows=4999, cols=1003, dtype="fp32", affine=2,
+        dict(name="norm, odd width", op="norm", rows=4999, cols=1003, dtype="fp32", affine=2,
              train=True),
         # --- log probabilities ----------------------------------------------
         # sampling or scoring one position of a large vocabulary, 20 alternatives
-        dict(name="logprobs one position", op="logprobs", rows=1, cols=129000, dtype="bf16",
+        dict(name="logprobs, one position", op="logprobs", rows=1, cols=129000, dtype="bf16",
              top=20, pad=0, masked=False, train=False),
         # an ImageNet head at the benchmark's batch: loss, entropy and the top 5
-        dict(name="logprobs classes", op="logprobs", rows=1536, cols=1000, dtype="fp32",
+        dict(name="logprobs, classes", op="logprobs", rows=1536, cols=1000, dtype="fp32",
              top=5, pad=0, masked=False, train=True),
         # training on a vocabulary of odd size held in padded rows
-        dict(name="logprobs padded rows", op="logprobs", rows=4095, cols=50001, dtype="bf16",
+        dict(name="logprobs, padded rows", op="logprobs", rows=4095, cols=50001, dtype="bf16",
              top=0, pad=47, masked=False, train=True),
         # a long batch on a large vocabulary, loss and entropy with their gradient
-        dict(name="logprobs large", op="logprobs", rows=8192, cols=131072, dtype="bf16",
+        dict(name="logprobs, large", op="logprobs", rows=8192, cols=131072, dtype="bf16",
              top=0, pad=0, masked=False, train=True),
         # --- GELU, its input kept in 8 bits ---------------------------------
         # a small layer: latency of the two passes
-        dict(name="gelu small", op="gelu", rows=256, cols=1024, dtype="bf16"),
+        dict(name="gelu, small", op="gelu", rows=256, cols=1024, dtype="bf16"),
         # the hidden rows of a large multi-layer perceptron
-        dict(name="gelu large", op="gelu", rows=16384, cols=8192, dtype="bf16"),
+        dict(name="gelu, large", op="gelu", rows=16384, cols=8192, dtype="bf16"),
         # a width that no vector load divides and a last block that is not full
-        dict(name="gelu odd width", op="gelu", rows=2047, cols=1111, dtype="fp16"),
+        dict(name="gelu, odd width", op="gelu", rows=2047, cols=1111, dtype="fp16"),
         # --- weight and bias gradient of a dense layer, input kept in 8 bits --
         # a large layer's backward: the matrix product counts
-        dict(name="dense large", op="dense", rows=16384, outs=4096, cols=4096, dtype="bf16"),
+        dict(name="dense, large", op="dense", rows=16384, outs=4096, cols=4096, dtype="bf16"),
         # few outputs, odd sizes: the long axis has to be split
-        dict(name="dense odd sizes", op="dense", rows=7999, outs=515, cols=1001, dtype="fp16"),
+        dict(name="dense, odd sizes", op="dense", rows=7999, outs=515, cols=1001, dtype="fp16"),
     ]
 
 
