@@ -502,13 +502,16 @@ struct D8WideArgs {
 };
 
 // 16 bytes per lane to LDS address lds (wave-uniform) + 16 * lane, from a uniform
-// base and 32-bit lane offsets, or from an address per lane
+// base and 32-bit lane offsets, or from an address per lane (s_nop: the wait state
+// between a scalar write of M0 and a load to LDS)
 __device__ __forceinline__ void dma16(const void* base, uint32_t off, uint32_t lds) {
-  asm volatile("s_mov_b32 m0, %2\n\tglobal_load_lds_dwordx4 %0, %1" ::"v"(off), "s"(base), "s"(lds)
+  asm volatile("s_mov_b32 m0, %2\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %0, %1" ::"v"(off),
+               "s"(base), "s"(lds)
                : "m0", "memory");
 }
 __device__ __forceinline__ void dma16_any(const void* src, uint32_t lds) {
-  asm volatile("s_mov_b32 m0, %1\n\tglobal_load_lds_dwordx4 %0, off" ::"v"(src), "s"(lds)
+  asm volatile("s_mov_b32 m0, %1\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %0, off" ::"v"(src),
+               "s"(lds)
                : "m0", "memory");
 }
 

@@ -29,12 +29,15 @@ __device__ __attribute__((aligned(256))) uint32_t g_ones_page_bf16[128] = {
 // front of the next ds_read, draining the ring every K-step; here the ring's
 // ordering is explicit (counted vmcnt + s_barrier, see the main loop).
 // M0 holds the wave-uniform LDS base; the compiler sets M0 itself before any
-// of its own M0 uses, so clobbering it here is safe.
+// of its own M0 uses, so clobbering it here is safe.  The s_nop is the one wait
+// state that a load to LDS needs behind a scalar write of M0; the compiler puts it
+// in by itself, but not inside an asm string.
 #pragma clang diagnostic ignored "-Winline-asm"
 __device__ __forceinline__ void glds16(const void* src, const void* lds_dst) {
   const uint32_t base = __builtin_amdgcn_readfirstlane(
       (uint32_t)(uintptr_t)(const __attribute__((address_space(3))) void*)lds_dst);
-  asm volatile("s_mov_b32 m0, %1\n\tglobal_load_lds_dwordx4 %0, off" ::"v"(src), "s"(base)
+  asm volatile("s_mov_b32 m0, %1\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %0, off" ::"v"(src),
+               "s"(base)
                : "m0");
 }
 #define ZK_GLDS16(src, dst) glds16((src), (dst))

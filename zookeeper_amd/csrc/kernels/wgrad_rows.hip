@@ -156,7 +156,9 @@ __device__ __forceinline__ __attribute__((address_space(3))) s16x4* lds_s16x4(
 
 // global_load_lds_dwordx4 into LDS byte address lds (wave-uniform: M0)
 __device__ __forceinline__ void glds16_at(const void* src, unsigned lds) {
-  asm volatile("s_mov_b32 m0, %1\n\tglobal_load_lds_dwordx4 %0, off" ::"v"(src), "s"(lds) : "m0");
+  asm volatile("s_mov_b32 m0, %1\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %0, off" ::"v"(src),
+               "s"(lds)
+               : "m0");
 }
 
 // 8 k-values of one column from two per-lane LDS addresses (rows q and q + 4
