@@ -470,3 +470,62 @@ def test_gradients_of_other_layouts():
             got, = torch.autograd.grad(dense8(x, w), w, dy)
             want, = torch.autograd.grad(dense8(x, w), w, dy.contiguous())
             assert torch.equal(got, want)
+
+
+def _form_of_small_steps(rows, cols):
+    """Codes of the whole range under the scale bytes 0 .. 8 (one to a row), which no
+    packed tensor has under 7 but other producers' forms do, and what they stand for
+    by the form's definition."""
+    from zookeeper_amd.ops import Packed8
+
+    g = torch.Generator().manual_seed(3)
+    codes = torch.randint(-127, 128, (rows, cols), generator=g, dtype=torch.int32).to(torch.int8)
+    scales = (torch.arange(rows).view(-1, 1) % 9).expand(rows, -(-cols // 32)).to(torch.uint8)
+    value = codes.double() * torch.exp2(scales[:, :1].double() - 133)
+    kept = Packed8(codes.cuda(), scales.contiguous().cuda(), torch.float32)
+    return kept, value.cuda()
+
+
+def test_small_steps_unpacked_and_in_gelu():
+    from zookeeper_amd.ops import unpack8
+    from zookeeper_amd.ops.act8 import _Gelu8Fn
+
+    kept, value = _form_of_small_steps(18, 100)
+    assert torch.equal(unpack8(kept, torch.float32).double(), value)
+    assert torch.equal(unpack8(kept, torch.bfloat16).double(), value)  # exact in bf16
+    assert torch.equal(unpack8(kept, torch.float16).double(), value.to(torch.float16).double())
+
+    class Ctx:
+        rows = 18
+        saved_tensors = (torch.cat([kept.codes.view(torch.uint8).reshape(-1),
+                                    kept.scales.reshape(-1)]),)
+
+    with torch.no_grad():
+        dx = _Gelu8Fn.backward(Ctx, torch.full((18, 100), 3.0, device="cuda"))
+    # the slope at |x| < 2^-117 is 1 / 2 + O(x): one rounding of Phi, of the sum and of
+    # the product each, the fit's 1e-7
+    assert ((dx - 1.5).abs() <= 1.5 * (1e-7 + 4 * 2.0 ** -24)).all()
+
+
+@pytest.mark.parametrize("variant", [0, 1])
+@pytest.mark.parametrize("dt", DTYPES)
+def test_small_steps_in_the_weight_gradient(dt, variant):
+    """Both kernels decode the same values; dy is scaled up so that the products are
+    normal numbers."""
+    from zookeeper_amd.ops.act8 import _dense_grads
+
+    rows, outs, cols = 189, 70, 130
+    kept, value = _form_of_small_steps(rows, cols)
+    torch.manual_seed(4)
+    up = 2.0 ** 14 if dt == torch.float16 else 2.0 ** 60
+    dy = (torch.randn(rows, outs, device="cuda").clamp(-3.9, 3.9) * up).to(dt)
+    dw, db = _dense_grads(dy, kept.codes, kept.scales, True, variant=variant)
+    d = dy.double()
+    want, mag = d.t() @ value, d.abs().t() @ value.abs()
+    # every product exact, a sum of them off by a rounding each (as above); fp16: a step
+    # of the subnormals each, where the sums fall under the normal range
+    tol = (rows + 16) * (2.0 ** -23 * mag + (2.0 ** -149 if dt == torch.float16 else 0))
+    assert ((dw.double() - want).abs() <= tol).all()
+    zero = torch.zeros_like(kept.codes)
+    dw, _ = _dense_grads(dy, zero, torch.zeros_like(kept.scales), True, variant=variant)
+    assert torch.equal(dw, torch.zeros_like(dw))

@@ -112,3 +112,15 @@ def test_refusals():
         v = x.clone().requires_grad_(True)
         torch.autograd.grad(gelu8(v).sum(), v, create_graph=True)
     assert math.isfinite(float(unpack8(k).sum()))
+
+
+def test_steps_under_the_smallest_packed_one():
+    """Scale bytes that pack8 does not write mean what the form says."""
+    scales = torch.arange(10, dtype=torch.uint8).view(10, 1)
+    codes = torch.tensor([[-127, -3, 0, 1, 64]] * 10, dtype=torch.int8)
+    want = codes.double() * torch.exp2(scales.double() - 133)
+    kept = Packed8(codes, scales, torch.float32)
+    assert torch.equal(unpack8(kept).double(), want)
+    assert torch.equal(unpack8(kept, torch.bfloat16).double(), want)
+    dw, _ = dense8_grads(torch.eye(10) * 2.0 ** 100, kept)
+    assert torch.equal(dw.double(), want * 2.0 ** 100)

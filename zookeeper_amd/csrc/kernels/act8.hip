@@ -7,7 +7,9 @@
 // OCP MXINT8 format).  E - 127 = floor(log2(max |x|)), one more where the largest
 // value would round to code 128 (so every value is within half a step; only E =
 // 254 clamps), never under E = 7 (step 2^-126: the smallest normal).  A block
-// that holds an infinity or a NaN has E = 255 and decodes to NaN.
+// that holds an infinity or a NaN has E = 255 and decodes to NaN.  E under 7, which
+// pack does not write but a form from elsewhere may hold (zeroed memory, for one),
+// decodes to its subnormal step; whole steps of that are exact in bf16 too.
 //
 // Why whole steps of a power of two and not e4m3: codes up to 127 and a sign are
 // exact in bf16, so a decoded tile feeds the bf16 matrix instructions without a
@@ -37,7 +39,7 @@ __device__ __forceinline__ uint32_t quad_max(uint32_t v) {
 }
 
 __device__ __forceinline__ float step_of(uint32_t E) {  // 2^(E - 133); E = 255: NaN
-  return E == 255u ? NAN : __uint_as_float((E < 7u ? 1u : E - 6u) << 23);
+  return E == 255u ? NAN : __uint_as_float(E < 7u ? 0x10000u << E : (E - 6u) << 23);
 }
 
 // The quad's block of 32: scale byte and this lane's 8 codes.
@@ -600,7 +602,8 @@ __global__ __launch_bounds__(kWNT, 2) void dense8_wide_kernel(D8WideArgs a) {
   const uint32_t xput = crow * 512 + (((tid & 31) ^ tr_swz<512>(crow)) << 4);
   auto put = [&](const Codes& c, int s, int h) {
     const uint32_t at = xput + kWX + (s & 1) * kWBuf + h * kWPiece;
-    const bool far_end = __any(max(c.e[0], c.e[1]) >= 254u);  // NaN blocks, largest steps
+    // NaN blocks, the largest steps (E >= 254) and subnormal ones (E < 7, which wraps)
+    const bool far_end = __any(max(c.e[0] - 7u, c.e[1] - 7u) >= 247u);
 #pragma unroll
     for (int i = 0; i < 2; ++i) {
       uint32_t b[2] = {c.w[i][0], c.w[i][1]};

@@ -87,9 +87,10 @@ def _empty_form(x):
 # --- the definitions in PyTorch (host tensors) --------------------------------
 
 def _steps(scales):
-    """2^(scale - 133) of each block, fp32; NaN for 255."""
+    """2^(scale - 133) of each block, fp32 (subnormal under 7); NaN for 255."""
     s = scales.to(torch.int32)
-    step = ((s - 6).clamp_min(1) << 23).view(torch.float32)
+    low = torch.ones_like(s) << (s.clamp_max(6) + 16)
+    step = torch.where(s < 7, low, (s - 6) << 23).view(torch.float32)
     return torch.where(s == 255, torch.full_like(step, float("nan")), step)
 
 
