@@ -294,3 +294,24 @@ def test_replays_in_a_graph():
         torch.cuda.synchronize()
         for a, e in zip(out, step(new)):
             assert torch.equal(a, e), k
+
+
+def test_the_longest_rows():
+    """The last split of a row of almost 2^31 logits ends past 2^31 - 1 when rounded up."""
+    from zookeeper_amd.ops import token_logprobs
+
+    V = 0x7FFF0000 - 1
+    x = torch.zeros(1, V, device="cuda", dtype=torch.bfloat16)
+    x[0, V - 1], x[0, V - 2], x[0, 5] = 25.0, 24.0, 23.0
+    r = token_logprobs(x, torch.tensor([V - 1], device="cuda"), top=4)
+    assert r.top_ids.tolist() == [[V - 1, V - 2, 5, 0]]
+    d = torch.tensor([0.0, -1.0, -2.0, -25.0], dtype=torch.float64)
+    n = torch.tensor([1.0, 1.0, 1.0, V - 3], dtype=torch.float64)
+    z = (n * d.exp()).sum()
+    lp = d - z.log()
+    # a thread adds V / (64 * 256) zeros' terms one after the other, each sum rounded; they
+    # are `share` of z.  The few other terms and joins: 200 u as above
+    share = float(n[3] * d[3].exp() / z)
+    tol = V / (64 * 256) * U * share + 200 * U
+    assert abs(float(r.logp[0]) - float(lp[0])) <= tol
+    assert ((r.top_logp[0].double().cpu() - lp).abs() <= tol + 4 * U * lp.abs()).all()

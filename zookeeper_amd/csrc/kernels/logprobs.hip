@@ -243,6 +243,11 @@ struct LpArgs {
   int V, k, splits, chunk;
 };
 
+// The last of 64 splits, each rounded up to 2048, may reach past 2^31 - 1.
+__device__ __forceinline__ int split_end(const LpArgs& a, int lo) {
+  return a.V - lo < a.chunk ? a.V : lo + a.chunk;
+}
+
 // One thread's answer for the row from its statistics.
 template <int DT>
 __device__ __forceinline__ float lp_finish(const LpArgs& a, long long row, const Stat& t) {
@@ -295,7 +300,7 @@ __global__ __launch_bounds__(kNT, 8) void lp_fwd_kernel(LpArgs a) {
   const long long row = a.row0 + (WPR == 1 ? unit : unit / a.splits);
   if (row >= a.rows) return;  // WPR = 1 only (no barrier below), or past the last row as a block
   const int split = WPR == 1 ? 0 : (int)(unit % a.splits);
-  const int lo = split * a.chunk, hi = min(a.V, lo + a.chunk);
+  const int lo = split * a.chunk, hi = split_end(a, lo);
   const raw* x = reinterpret_cast<const raw*>(a.x) + row * a.xs;
   Stat st{-INFINITY, 0.f, 0.f};
   Top top = top_new(a.k, lds + (TOP ? wave * 128 : 0));
@@ -451,7 +456,7 @@ __global__ __launch_bounds__(kNT) void lp_bwd_kernel(LpArgs a) {
   const long long row = a.row0 + (WPR == 1 ? unit : unit / a.splits);
   if (row >= a.rows) return;
   const int split = WPR == 1 ? 0 : (int)(unit % a.splits);
-  const int lo = split * a.chunk, hi = min(a.V, lo + a.chunk);
+  const int lo = split * a.chunk, hi = split_end(a, lo);
   const raw* x = reinterpret_cast<const raw*>(a.x) + row * a.xs;
   raw* dx = reinterpret_cast<raw*>(a.dx) + row * a.V;
   const float m = a.stats[row * 3], ls = a.stats[row * 3 + 1], h = a.stats[row * 3 + 2];
