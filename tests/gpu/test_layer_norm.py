@@ -280,3 +280,29 @@ def test_gradients_of_other_layouts():
             got = torch.autograd.grad(layer_norm(x, w), [x, w], dy)
             want = torch.autograd.grad(layer_norm(x, w), [x, w], dy.contiguous())
             assert all(torch.equal(a, b) for a, b in zip(got, want))
+
+
+@pytest.mark.parametrize("cols", [1, 2, 4, 8, 64, 4096, 32768])
+@pytest.mark.parametrize("dt", [torch.float32, torch.bfloat16])
+def test_large_constant_rows(cols, dt):
+    """Rows of one large value and a small eps: xhat is 0 and dx the gradient without its
+    mean, also where the width does not fill the lanes."""
+    from zookeeper_amd.ops import layer_norm
+
+    # powers of two: the sum, the mean and the differences of 0 are exact
+    torch.manual_seed(9)
+    x = torch.full((3, cols), 2.0 ** 112, device="cuda", dtype=dt)
+    x[1] = -x[1]
+    x.requires_grad_(True)
+    w = torch.rand(cols, device="cuda", requires_grad=True)
+    dy = torch.randn(3, cols, device="cuda").to(dt)
+    y = layer_norm(x, w, eps=1e-12)  # xhat of a 0 would be 2^112 * 1e6: an infinity
+    assert torch.equal(y, torch.zeros_like(y))
+    dx, dw = torch.autograd.grad(y, [x, w], dy)
+    assert torch.equal(dw, torch.zeros_like(dw))
+    g = dy.double() * w.double()
+    want = (g - g.mean(-1, keepdim=True)) * 1e6
+    mag = (g.abs() + g.abs().mean(-1, keepdim=True)) * 1e6
+    # rstd, the products, the sum's n / 256 + 16 additions and two more roundings; the store
+    tol = (cols / 256 + 32) * U32 * mag + _half(dt) * want.abs()
+    assert ((dx.double() - want).abs() <= tol).all()

@@ -212,7 +212,7 @@ __global__ __launch_bounds__(block_of(G)) void ln_bwd_kernel(LnArgs a) {
     for (int k = 0; k < NV; ++k) {
       const int c = (k * G + l) * 8;
       nx[k] = raw8<DT>(x + c, a.D - c);
-      ny[k] = raw8<DT>(dy + c, a.D - c);  // zeros behind D: no share in any sum
+      ny[k] = raw8<DT>(dy + c, a.D - c);  // zeros behind D
     }
     nm = a.mean[r];
     nr = a.rstd[r];
@@ -231,6 +231,15 @@ __global__ __launch_bounds__(block_of(G)) void ln_bwd_kernel(LnArgs a) {
         g[k][i] = raw_at<DT>(ny[k], i);
       }
     const float mean = nm, rstd = nr;
+    // behind D: xhat 0 (a zero's own could overflow, and 0 * inf reach the sums)
+#pragma unroll
+    for (int k = 0; k < NV; ++k) {
+      const int n = a.D - (k * G + l) * 8;
+      if (n < 8)
+#pragma unroll
+        for (int i = 0; i < 8; ++i)
+          if (i >= n) xh[k][i] = mean;
+    }
     if (AHEAD && row + stride < a.rows) load(row + stride);
     float s1 = 0.f, s2 = 0.f;
 #pragma unroll
