@@ -315,3 +315,24 @@ def test_the_longest_rows():
     tol = V / (64 * 256) * U * share + 200 * U
     assert abs(float(r.logp[0]) - float(lp[0])) <= tol
     assert ((r.top_logp[0].double().cpu() - lp).abs() <= tol + 4 * U * lp.abs()).all()
+
+
+@pytest.mark.parametrize("V", [50, 5000])
+def test_the_entropy_does_not_depend_on_the_token(V):
+    """... nor does its gradient, on the host either."""
+    from zookeeper_amd.ops import token_logprobs
+
+    x, t = _inputs(6, V, torch.float32, 1)
+    x.requires_grad_(True)
+    want, = torch.autograd.grad(token_logprobs(x, t).entropy.sum(), x)
+    t[1], t[2], t[3] = -100, -1, V
+    r = token_logprobs(x, t)
+    assert r.logp[2:4].isnan().all()
+    assert torch.equal(torch.autograd.grad(r.entropy.sum(), x)[0], want)
+    host = x.detach().cpu().requires_grad_(True)
+    dx, = torch.autograd.grad(token_logprobs(host, t.cpu()).entropy.sum(), host)
+    assert torch.isfinite(dx).all()
+    # with the log probability's too, the NaN is in its own rows only
+    r = token_logprobs(x, t)
+    dx, = torch.autograd.grad((r.logp + r.entropy).sum(), x)
+    assert dx[2:4].isnan().all() and torch.isfinite(dx[[0, 1, 4, 5]]).all()

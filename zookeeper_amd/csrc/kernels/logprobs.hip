@@ -37,7 +37,7 @@
 //
 // Rows: all -inf -> logp -inf, entropy 0, gradient 0.  A NaN or +inf -> NaN.
 // The ignored index: logp 0 and no gradient from it.  Any other token outside
-// [0, V): logp NaN and a NaN gradient row.
+// [0, V): logp NaN, and a NaN gradient row if logp has a gradient.
 #include "rows.h"
 
 namespace {
@@ -465,7 +465,7 @@ __global__ __launch_bounds__(kNT) void lp_bwd_kernel(LpArgs a) {
   const float gh = a.g_entropy ? a.g_entropy[row] : 0.f;
   const bool in = tok >= 0 && tok < a.V;
   if (tok == a.ignore) gl = 0.f;
-  else if (!in) gl = NAN;
+  else if (!in && a.g_logp) gl = NAN;
   const bool none = m == -INFINITY && ls == 0.f;
   const float ga = gl + gh * h;
   const int t = in ? (int)tok : -1;

@@ -15,9 +15,10 @@ The alternatives are for reporting and carry no gradient.
   probability 0 without gradient; the row's entropy is not affected.
 * Masked logits are ``-inf``: probability 0, no share in the entropy.  A row of
   nothing but ``-inf`` has log probability ``-inf``, entropy 0, gradient 0.
-* Any other token outside ``[0, V)`` gives NaN, as does a row with a NaN or
-  ``+inf`` (a NaN ranks above all numbers among the alternatives); the gradient
-  row is NaN then.
+* Any other token outside ``[0, V)`` gives a log probability of NaN, whose gradient
+  makes the row's NaN; the entropy and its gradient do not depend on the token.
+* A row with a NaN or ``+inf`` gives NaN for both and a NaN gradient row (a NaN ranks
+  above all numbers among the alternatives).
 """
 
 from __future__ import annotations
