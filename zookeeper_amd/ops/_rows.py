@@ -17,8 +17,9 @@ from zookeeper_amd.ops import _native
 DTYPE_CODES = {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2}
 _FLOATS = (torch.float32, torch.bfloat16, torch.float16, torch.float64)
 
-# Raw hipStream_t of torch's current stream on a device index.
-raw_stream = torch._C._cuda_getCurrentRawStream
+# Raw hipStream_t of torch's current stream on a device index (a torch without GPU
+# support lacks the name, and has no GPU tensors to need it).
+raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None)
 
 _HERE = contextlib.nullcontext()
 
