@@ -279,3 +279,52 @@ def test_a_dropped_graph_does_not_hold_back_a_parameter():
     y.backward(retain_graph=True)
     y.backward()
     assert len(count) == 3 * len(flat.slots)
+
+
+def _operators():
+    from zookeeper_amd import ops
+
+    t = torch.randint(0, 100, (40,), generator=torch.Generator().manual_seed(1)).cuda()
+    w = torch.rand(100, device="cuda")
+    return [lambda v: ops.layer_norm(v, w), ops.gelu8,
+            lambda v: ops.token_logprobs(v, t, top=3)[:3], lambda v: ops.dense8(v, w[None])]
+
+
+@pytest.mark.parametrize("recorded", [False, True])
+def test_traced_calls_are_run_again(recorded):
+    """A trace without gradients holds the operators and not their empty outputs."""
+    torch.manual_seed(8)
+    x = torch.randn(40, 100, device="cuda", requires_grad=recorded)
+    for f in _operators():
+        traced = torch.jit.trace(f, (x,), check_trace=False)
+        for _ in range(2):
+            z = torch.randn(40, 100, device="cuda")
+            got, want = traced(z), f(z)
+            if isinstance(got, torch.Tensor):
+                got, want = (got,), (want,)
+            assert all(torch.equal(a, b) for a, b in zip(got, want))
+
+
+def test_forms_are_not_traced():
+    from zookeeper_amd import ops
+
+    x = torch.randn(8, 64, device="cuda")
+    kept = ops.pack8(x)
+    for f in (lambda v: ops.pack8(v).codes, lambda v: v + ops.unpack8(kept),
+              lambda v: ops.dense8_grads(v, kept)[0]):
+        with pytest.raises(RuntimeError, match="traced"):
+            torch.jit.trace(f, (x,), check_trace=False)
+
+
+def test_forward_mode_is_refused():
+    from torch.autograd import forward_ad
+
+    x = torch.randn(40, 100, device="cuda")
+    with forward_ad.dual_level():
+        dual = forward_ad.make_dual(x, torch.ones_like(x))
+        for f in _operators()[:3]:  # dense8 without a recorded weight is torch's product
+            with pytest.raises(NotImplementedError, match="jvp"):
+                f(dual)
+            with pytest.raises(NotImplementedError, match="jvp"), torch.no_grad():
+                f(dual)
+            f(x)  # no tangent: as always

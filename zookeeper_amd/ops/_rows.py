@@ -10,6 +10,7 @@ import weakref
 from typing import Dict, Optional, Tuple
 
 import torch
+from torch.autograd import forward_ad
 
 from zookeeper_amd.ops import _native
 
@@ -46,6 +47,18 @@ def use_kernels(t: torch.Tensor, what: str) -> bool:
     return True
 
 
+def tracked() -> bool:
+    """True while torch follows calls by other means than ``requires_grad``: tracing
+    records an autograd function as one call, and forward-mode differentiation
+    is refused by it.  A bare launch would be invisible to both."""
+    return forward_ad._current_level >= 0 or torch._C._is_tracing()
+
+
+def refuse_tracing(what: str) -> None:
+    if torch._C._is_tracing():
+        raise RuntimeError(f"{what}: cannot be traced (it is no autograd function)")
+
+
 def guard(t: torch.Tensor):
     """Context that makes ``t``'s device the current one for a launch."""
     if t.device.index == torch._C._cuda_getDevice():
@@ -56,15 +69,16 @@ def guard(t: torch.Tensor):
 def rows_of(t: torch.Tensor) -> Tuple[torch.Tensor, int, int]:
     """``(t2, rows, row stride)``: ``t`` as rows of its last dimension with unit
     stride inside a row -- a view where the strides allow it (padded, sliced or
-    broadcast rows), a contiguous copy otherwise."""
-    cols = t.shape[-1]
+    broadcast rows), a contiguous copy otherwise.  ``int``: sizes are tensors
+    while a call is traced."""
+    cols = int(t.shape[-1])
     if t.is_contiguous():
-        return t, t.numel() // cols if cols else 0, cols
+        return t, int(t.numel()) // cols if cols else 0, cols
     if t.dim() != 2:
         t = t.reshape(-1, cols)
     if cols > 1 and t.stride(1) != 1:
         t = t.contiguous()
-    return t, t.shape[0], t.stride(0)
+    return t, int(t.shape[0]), int(t.stride(0))
 
 
 def check_param(p, cols: int, x: torch.Tensor, what: str) -> None:

@@ -31,8 +31,8 @@ import torch.nn.functional as F
 
 from zookeeper_amd.ops._native import lib
 from zookeeper_amd.ops._rows import (DTYPE_CODES, call, flat_grad, guard, last_use_ready,
-                                     note_uses, ptr, raw_stream, refuse_twice, rows_of,
-                                     use_kernels)
+                                     note_uses, ptr, raw_stream, refuse_tracing, refuse_twice,
+                                     rows_of, tracked, use_kernels)
 
 BLOCK = 32
 
@@ -79,7 +79,7 @@ def _check_input(x: torch.Tensor, what: str) -> None:
 
 def _empty_form(x):
     codes = torch.empty(x.shape, dtype=torch.int8, device=x.device)
-    scales = torch.empty((*x.shape[:-1], -(-x.shape[-1] // BLOCK)), dtype=torch.uint8,
+    scales = torch.empty((*x.shape[:-1], -(-int(x.shape[-1]) // BLOCK)), dtype=torch.uint8,
                          device=x.device)
     return codes, scales
 
@@ -123,18 +123,23 @@ def _gelu_slope(k):
 
 # --- pack / unpack --------------------------------------------------------------
 
+def _pack(x):
+    codes, scales = _empty_form(x)
+    x2, rows, stride = rows_of(x)
+    with guard(x):
+        call(lib().zk_pack8, "zk_pack8", x2.data_ptr(), codes.data_ptr(), scales.data_ptr(), rows,
+             int(x.shape[-1]), stride, DTYPE_CODES[x.dtype], raw_stream(x.device.index))
+    return codes, scales
+
+
 def pack8(x: torch.Tensor) -> Packed8:
     """The 8-bit form of ``x`` (fp32, bf16 or fp16 on the GPU; any leading shape
     and row stride).  Not differentiable: the form is what a backward keeps."""
     _check_input(x, "pack8")
     if not use_kernels(x, "pack8"):
         return Packed8(*_pack_plain(x), x.dtype)
-    codes, scales = _empty_form(x)
-    x2, rows, stride = rows_of(x)
-    with guard(x):
-        call(lib().zk_pack8, "zk_pack8", x2.data_ptr(), codes.data_ptr(), scales.data_ptr(), rows,
-             x.shape[-1], stride, DTYPE_CODES[x.dtype], raw_stream(x.device.index))
-    return Packed8(codes, scales, x.dtype)
+    refuse_tracing("pack8")
+    return Packed8(*_pack(x), x.dtype)
 
 
 def unpack8(kept: Packed8, dtype: Optional[torch.dtype] = None) -> torch.Tensor:
@@ -144,6 +149,7 @@ def unpack8(kept: Packed8, dtype: Optional[torch.dtype] = None) -> torch.Tensor:
     out = torch.empty(kept.shape, dtype=dtype, device=kept.device)
     if not use_kernels(out, "unpack8"):
         return _unpack_plain(kept.codes, kept.scales, dtype)
+    refuse_tracing("unpack8")
     n = kept.shape[-1]
     with guard(out):
         call(lib().zk_unpack8, "zk_unpack8", kept.codes.data_ptr(), kept.scales.data_ptr(),
@@ -157,7 +163,7 @@ def unpack8(kept: Packed8, dtype: Optional[torch.dtype] = None) -> torch.Tensor:
 def _gelu_forward(x, keep: bool):
     """``y`` and the kept input in one buffer: the codes, then the scales."""
     x2, rows, stride = rows_of(x)
-    n = x.shape[-1]
+    n = int(x.shape[-1])
     dev = x.device
     y = torch.empty_like(x) if x.is_contiguous() else torch.empty(x.shape, dtype=x.dtype,
                                                                   device=dev)
@@ -219,7 +225,9 @@ def gelu8(x: torch.Tensor) -> torch.Tensor:
     native = use_kernels(x, "gelu8")
     if x.requires_grad and torch.is_grad_enabled():
         return _Gelu8Fn.apply(x) if native else _Gelu8HostFn.apply(x)
-    return _gelu_forward(x, False)[0] if native else F.gelu(x)
+    if not native:
+        return F.gelu(x)
+    return _Gelu8Fn.apply(x) if tracked() else _gelu_forward(x, False)[0]
 
 
 # --- dense ------------------------------------------------------------------------
@@ -263,7 +271,8 @@ def dense8_grads(dy: torch.Tensor, kept: Packed8,
     row stride) and the kept input [..., K].
 
     bf16 gradients take one matrix product, fp16 and fp32 gradients two and
-    three (their exact bf16 terms); sums are fp32 in a fixed order."""
+    three (their exact bf16 terms); sums are fp32 in a fixed order.  Not
+    differentiable."""
     _check_input(dy, "dense8_grads")
     if dy.shape[:-1] != kept.shape[:-1]:
         raise ValueError(f"dense8_grads: rows differ: dy {tuple(dy.shape)}, "
@@ -272,6 +281,7 @@ def dense8_grads(dy: torch.Tensor, kept: Packed8,
         raise ValueError(f"dense8_grads: dy on {dy.device}, the kept input on {kept.device}")
     dy = dy.detach()
     if use_kernels(dy, "dense8_grads"):
+        refuse_tracing("dense8_grads")
         return _dense_grads(dy, kept.codes, kept.scales, bias)
     d = dy.reshape(-1, dy.shape[-1]).float()
     x = _unpack_plain(kept.codes, kept.scales, torch.float32).reshape(-1, kept.shape[-1])
@@ -285,8 +295,7 @@ class _Dense8Fn(torch.autograd.Function):
         y = F.linear(x, w, bias.to(x.dtype) if bias is not None else None)
         codes = scales = None
         if ctx.needs_input_grad[1]:
-            kept = pack8(x)
-            codes, scales = kept.codes, kept.scales
+            codes, scales = _pack(x) if use_kernels(x, "dense8") else _pack_plain(x)
         ctx.save_for_backward(codes, scales, weight)
         ctx.weight_param, ctx.bias_param = weight, bias
         ctx.uses = note_uses(weight, bias)

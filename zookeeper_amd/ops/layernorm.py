@@ -22,7 +22,7 @@ import torch
 from zookeeper_amd.ops._native import lib
 from zookeeper_amd.ops._rows import (DTYPE_CODES, as_fp32, call, check_param, flat_grad, guard,
                                      last_use_ready, note_uses, ptr, raw_stream, refuse_twice,
-                                     rows_of, use_kernels)
+                                     rows_of, tracked, use_kernels)
 
 
 @functools.lru_cache(maxsize=256)
@@ -44,7 +44,7 @@ def _forward(x, weight, bias, eps: float, stats: bool):
     w, b = as_fp32(weight), as_fp32(bias)
     with guard(x):
         call(lib().zk_layer_norm_fwd, "zk_layer_norm_fwd", x2.data_ptr(), ptr(w), ptr(b),
-             y.data_ptr(), mean, rstd, rows, x.shape[-1], stride, eps, DTYPE_CODES[x.dtype],
+             y.data_ptr(), mean, rstd, rows, int(x.shape[-1]), stride, eps, DTYPE_CODES[x.dtype],
              raw_stream(dev.index))
     return y, st
 
@@ -148,8 +148,8 @@ def layer_norm(x: torch.Tensor, weight: Optional[torch.Tensor] = None,
         return _plain(x, weight, bias, eps)
     if x.shape[-1] >= 1 << 31 or x.numel() // x.shape[-1] >= 1 << 31:
         raise ValueError(f"layer_norm: at most 2^31 - 1 rows and columns, got {tuple(x.shape)}")
-    if torch.is_grad_enabled() and (x.requires_grad
-                                    or (weight is not None and weight.requires_grad)
-                                    or (bias is not None and bias.requires_grad)):
+    if tracked() or torch.is_grad_enabled() and (
+            x.requires_grad or (weight is not None and weight.requires_grad)
+            or (bias is not None and bias.requires_grad)):
         return _LayerNormFn.apply(x, weight, bias, eps)
     return _forward(x, weight, bias, eps, False)[0]

@@ -29,7 +29,7 @@ import torch
 
 from zookeeper_amd.ops._native import lib
 from zookeeper_amd.ops._rows import (DTYPE_CODES, call, guard, ptr, raw_stream, refuse_twice,
-                                     rows_of, use_kernels)
+                                     rows_of, tracked, use_kernels)
 
 MAX_TOP = 64
 
@@ -42,7 +42,7 @@ class TokenLogProbs(NamedTuple):
 
 
 def _forward(logits, tokens, top: int, ignore: int, keep: bool):
-    dev, lead, V = logits.device, logits.shape[:-1], logits.shape[-1]
+    dev, lead, V = logits.device, logits.shape[:-1], int(logits.shape[-1])
     x, rows, stride = rows_of(logits)
     L = lib()
     f32 = torch.float32
@@ -151,6 +151,6 @@ def token_logprobs(logits: torch.Tensor, tokens: torch.Tensor, top: int = 0,
     if logits.shape[-1] >= 0x7FFF0000:
         raise ValueError(f"token_logprobs: rows of {logits.shape[-1]} elements are too long")
     tokens = tokens.contiguous()
-    if logits.requires_grad and torch.is_grad_enabled():
+    if tracked() or logits.requires_grad and torch.is_grad_enabled():
         return TokenLogProbs(*_TokenLogProbsFn.apply(logits, tokens, top, ignore_index))
     return TokenLogProbs(*_forward(logits, tokens, top, ignore_index, False)[:4])
