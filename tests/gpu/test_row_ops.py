@@ -328,3 +328,21 @@ def test_forward_mode_is_refused():
             with pytest.raises(NotImplementedError, match="jvp"), torch.no_grad():
                 f(dual)
             f(x)  # no tangent: as always
+
+
+def test_a_module_is_saved_whole_after_data_parallel_steps(tmp_path):
+    model, flat = _shared_model()
+    for slot in flat.slots:
+        slot.param._zk_grad_ready = _nothing
+    x = torch.randn(8, 64, device="cuda")
+    z = model(model(x)).sum()
+    z.backward()
+    for slot in flat.slots:  # as the bucketer does at its end
+        del slot.param._zk_grad_ready
+    torch.save(model, tmp_path / "model.pt")
+    again = torch.load(tmp_path / "model.pt", weights_only=False)
+    assert torch.equal(again(again(x)).sum(), z)
+
+
+def _nothing():
+    pass

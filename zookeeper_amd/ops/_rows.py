@@ -106,7 +106,16 @@ def ptr(t):
 class _Use:
     """One recorded use of a parameter whose gradient is still to come."""
 
-    __slots__ = ("__weakref__",)
+    __slots__ = ("param", "__weakref__")
+
+    def __init__(self, param):
+        self.param = param
+
+
+# Recorded uses by parameter (a use holds its parameter, so an id means one while any is
+# left).  Not kept on the parameter itself: a module is saved with its parameters'
+# attributes.
+_USES: Dict[int, "weakref.WeakSet[_Use]"] = {}
 
 
 def note_uses(*params):
@@ -117,8 +126,8 @@ def note_uses(*params):
     for p in params:
         token = None
         if p is not None and getattr(p, "_zk_grad_ready", None) is not None:
-            token = _Use()
-            p.__dict__.setdefault("_zk_uses", weakref.WeakSet()).add(token)
+            token = _Use(p)
+            _USES.setdefault(id(p), weakref.WeakSet()).add(token)
         tokens.append(token)
     return tokens
 
@@ -127,10 +136,12 @@ def last_use_ready(p, token) -> None:
     """Backward: tell the bucketer that ``p``'s gradient is complete, once no
     other recorded use of ``p`` is to come (a layer applied twice)."""
     if token is not None:
-        uses = p.__dict__["_zk_uses"]
-        uses.discard(token)
+        uses = _USES.get(id(p), ())
+        if uses:
+            uses.discard(token)
         if uses:
             return
+        _USES.pop(id(p), None)
     _native.grad_ready(p)
 
 
