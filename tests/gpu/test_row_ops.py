@@ -346,3 +346,26 @@ def test_a_module_is_saved_whole_after_data_parallel_steps(tmp_path):
 
 def _nothing():
     pass
+
+
+def test_a_graph_passed_twice_reports_complete_gradients():
+    """The same layers twice in one graph, and two passes over it."""
+    model, flat = _shared_model()
+    x = torch.randn(16, 64, device="cuda")
+    z = model(model(x)).square().sum()
+    flat.zero_grad()
+    z.backward(retain_graph=True)
+    torch.cuda.synchronize()
+    want = flat.grad.clone()
+    seen = []
+    for slot in flat.slots:
+        slot.param._zk_grad_ready = lambda slot=slot: seen.append((slot,
+                                                                   slot.param.grad.clone()))
+    for _ in range(2):
+        flat.zero_grad()
+        seen.clear()
+        z.backward(retain_graph=True)
+        torch.cuda.synchronize()
+        assert torch.equal(flat.grad, want)
+        assert sorted(s.name for s, _ in seen) == sorted(s.name for s in flat.slots)
+        assert all(torch.equal(g, s.param.grad) for s, g in seen)

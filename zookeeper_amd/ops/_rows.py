@@ -7,7 +7,7 @@ from __future__ import annotations
 
 import contextlib
 import weakref
-from typing import Dict, Optional, Tuple
+from typing import Dict, Optional, Set, Tuple
 
 import torch
 from torch.autograd import forward_ad
@@ -103,50 +103,31 @@ def ptr(t):
     return None if t is None else t.data_ptr()
 
 
-class _Use:
-    """One recorded use of a parameter whose gradient is still to come."""
+# --- flat gradients ------------------------------------------------------------
 
-    __slots__ = ("param", "__weakref__")
+class _Pass:
+    """The flat gradients written in one backward pass: the stream of each
+    parameter's last write, and the parameters written by uses that were recorded
+    inside of another pass.  Called at the pass's end by autograd's engine, which
+    holds the only lasting reference to it."""
 
-    def __init__(self, param):
-        self.param = param
+    __slots__ = ("writers", "inner", "__weakref__")
 
+    def __init__(self):
+        self.writers: Dict[int, Tuple[torch.device, int]] = {}
+        self.inner: Set[int] = set()
 
-# Recorded uses by parameter (a use holds its parameter, so an id means one while any is
-# left).  Not kept on the parameter itself: a module is saved with its parameters'
-# attributes.
-_USES: Dict[int, "weakref.WeakSet[_Use]"] = {}
-
-
-def note_uses(*params):
-    """Forward: a token for each parameter a data-parallel bucketer waits for
-    (None otherwise).  A token lives as long as the recorded graph, so a graph
-    that is dropped without a backward leaves none behind."""
-    tokens = []
-    for p in params:
-        token = None
-        if p is not None and getattr(p, "_zk_grad_ready", None) is not None:
-            token = _Use(p)
-            _USES.setdefault(id(p), weakref.WeakSet()).add(token)
-        tokens.append(token)
-    return tokens
+    def __call__(self):
+        for device, raw in set(self.writers.values()):
+            if raw != _raw(device):
+                torch.cuda.current_stream(device).wait_stream(_stream(device, raw))
 
 
-def last_use_ready(p, token) -> None:
-    """Backward: tell the bucketer that ``p``'s gradient is complete, once no
-    other recorded use of ``p`` is to come (a layer applied twice)."""
-    if token is not None:
-        uses = _USES.get(id(p), ())
-        if uses:
-            uses.discard(token)
-        if uses:
-            return
-        _USES.pop(id(p), None)
-    _native.grad_ready(p)
+_PASSES: "weakref.WeakValueDictionary[int, _Pass]" = weakref.WeakValueDictionary()
 
 
-# Streams that added into flat gradients, by backward pass and parameter.
-_WRITERS: Dict[int, Dict[int, Tuple[torch.device, int]]] = {}
+def _raw(device: torch.device) -> int:
+    return raw_stream(device.index) if device.type == "cuda" else 0
 
 
 def _stream(device: torch.device, raw: int):
@@ -155,33 +136,70 @@ def _stream(device: torch.device, raw: int):
     return torch.cuda.ExternalStream(raw, device)
 
 
-def _join_writers(task: int) -> None:
-    for device, raw in set(_WRITERS.pop(task, {}).values()):
-        if raw != raw_stream(device.index):
-            torch.cuda.current_stream(device).wait_stream(_stream(device, raw))
+def _accumulated(p) -> None:
+    """Autograd's hook behind the last use of ``p`` in a backward pass, whichever
+    uses that pass has: every write into its flat gradient is enqueued, each behind
+    the one before, so the bucketer may have it from the last one's stream on."""
+    current = _PASSES.get(torch._C._current_graph_task_id())
+    last = current.writers.get(id(p)) if current is not None else None
+    if last is None or id(p) in current.inner:
+        return
+    if last[1] == _raw(last[0]):
+        _native.grad_ready(p)
+    else:
+        with torch.cuda.stream(_stream(*last)):
+            _native.grad_ready(p)
 
 
-def flat_grad(p) -> Optional[torch.Tensor]:
-    """:func:`_native.direct_grad` for a parameter that may be used on several
-    streams in one backward pass.  Autograd orders the gradients it accumulates
-    and knows nothing of these: each write waits for the one before it on
-    another stream, and the caller's stream for all of them at the pass's end."""
+def in_backward() -> bool:
+    """True inside a backward pass.  A use recorded there belongs to a pass of its own
+    inside that one (reentrant checkpointing), and others may follow."""
+    return torch._C._current_graph_task_id() >= 0
+
+
+def flat_grad(p, inner: bool) -> Optional[torch.Tensor]:
+    """:func:`_native.direct_grad` for a parameter that may be used several times in
+    one backward pass, on several streams.  Autograd orders the gradients it
+    accumulates and knows nothing of these: each write waits for the one before it
+    on another stream, and the caller's stream for all of them at the pass's end.
+
+    The data-parallel bucketer hears of ``p`` once autograd is through with its last
+    use of the pass (:func:`_accumulated`); ``inner`` (a use recorded in a backward
+    pass): not before the bucketer's own end, as only that knows that no further
+    inner pass follows.  A write that comes too late all the same raises."""
     g = _native.direct_grad(p)
     if g is None:
         return None
+    ready = getattr(p, "_zk_grad_ready", None)
+    if getattr(ready, "launched", False):
+        raise RuntimeError(
+            "a gradient is written after its all-reduce was launched: the layer is used outside "
+            "and inside of a reentrant checkpoint, or twice before the bucketer's finish()")
     task = torch._C._current_graph_task_id()
     if task < 0:  # not inside a backward pass: one stream, the caller's
         return g
-    writers = _WRITERS.get(task)
-    if writers is None:
-        writers = _WRITERS[task] = {}
-        torch.autograd.Variable._execution_engine.queue_callback(lambda: _join_writers(task))
-    here = (g.device, raw_stream(g.device.index))
-    last = writers.get(id(p), here)
-    writers[id(p)] = here
+    current = _PASSES.get(task)
+    if current is None:
+        current = _PASSES[task] = _Pass()
+        torch.autograd.Variable._execution_engine.queue_callback(current)
+    here = (g.device, _raw(g.device))
+    last = current.writers.get(id(p), here)
+    current.writers[id(p)] = here
     if last != here:
         torch.cuda.current_stream(g.device).wait_stream(_stream(*last))
+    if inner:
+        current.inner.add(id(p))
+    elif ready is not None:
+        hooks = p._post_accumulate_grad_hooks
+        if hooks is None or _accumulated not in hooks.values():
+            p.register_post_accumulate_grad_hook(_accumulated)
     return g
+
+
+def written(p) -> None:
+    """After a write into ``p``'s flat gradient outside of any backward pass."""
+    if torch._C._current_graph_task_id() < 0:
+        _native.grad_ready(p)
 
 
 def refuse_twice(what: str) -> None:

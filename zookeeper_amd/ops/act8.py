@@ -30,9 +30,9 @@ import torch
 import torch.nn.functional as F
 
 from zookeeper_amd.ops._native import lib
-from zookeeper_amd.ops._rows import (DTYPE_CODES, call, flat_grad, guard, last_use_ready,
-                                     note_uses, ptr, raw_stream, refuse_tracing, refuse_twice,
-                                     rows_of, tracked, use_kernels)
+from zookeeper_amd.ops._rows import (DTYPE_CODES, call, flat_grad, guard, in_backward, ptr,
+                                     raw_stream, refuse_tracing, refuse_twice, rows_of, tracked,
+                                     use_kernels, written)
 
 BLOCK = 32
 
@@ -298,7 +298,7 @@ class _Dense8Fn(torch.autograd.Function):
             codes, scales = _pack(x) if use_kernels(x, "dense8") else _pack_plain(x)
         ctx.save_for_backward(codes, scales, weight)
         ctx.weight_param, ctx.bias_param = weight, bias
-        ctx.uses = note_uses(weight, bias)
+        ctx.inner = in_backward()
         return y
 
     @staticmethod
@@ -308,12 +308,11 @@ class _Dense8Fn(torch.autograd.Function):
         codes, scales, weight = ctx.saved_tensors
         need_x, need_w, need_b = ctx.needs_input_grad
         wp, bp = ctx.weight_param, ctx.bias_param
-        wuse, buse = ctx.uses
         dx = torch.matmul(dy, weight.to(dy.dtype)) if need_x else None
         dw = db = None
         native = use_kernels(dy, "dense8")
-        dw_direct = flat_grad(wp) if need_w and native else None
-        db_direct = flat_grad(bp) if need_b and native else None
+        dw_direct = flat_grad(wp, ctx.inner) if need_w and native else None
+        db_direct = flat_grad(bp, ctx.inner) if need_b and native else None
         if need_w and native:
             dw, db = _dense_grads(dy, codes, scales, need_b, dw_direct, db_direct)
         elif need_w:
@@ -323,12 +322,12 @@ class _Dense8Fn(torch.autograd.Function):
             if db_direct is not None:
                 db_direct += db
         if dw_direct is not None:
-            last_use_ready(wp, wuse)
+            written(wp)
             dw = None
         elif dw is not None:
             dw = dw.to(wp.dtype)
         if db_direct is not None:
-            last_use_ready(bp, buse)
+            written(bp)
             db = None
         elif db is not None:
             db = db.to(bp.dtype)

@@ -21,8 +21,8 @@ import torch
 
 from zookeeper_amd.ops._native import lib
 from zookeeper_amd.ops._rows import (DTYPE_CODES, as_fp32, call, check_param, flat_grad, guard,
-                                     last_use_ready, note_uses, ptr, raw_stream, refuse_twice,
-                                     rows_of, tracked, use_kernels)
+                                     in_backward, ptr, raw_stream, refuse_twice, rows_of, tracked,
+                                     use_kernels, written)
 
 
 @functools.lru_cache(maxsize=256)
@@ -58,7 +58,7 @@ class _LayerNormFn(torch.autograd.Function):
         y, stats = _forward(x, weight, bias, eps, True)
         ctx.save_for_backward(x, weight)
         # the parameters themselves: the flat gradient buffer hangs on them
-        ctx.rest = (stats, weight, bias, *note_uses(weight, bias))
+        ctx.rest = (stats, weight, bias, in_backward())
         return y
 
     @staticmethod
@@ -66,7 +66,7 @@ class _LayerNormFn(torch.autograd.Function):
         if torch.is_grad_enabled():
             refuse_twice("layer_norm")
         x, weight = ctx.saved_tensors
-        stats, wp, bp, wuse, buse = ctx.rest
+        stats, wp, bp, inner = ctx.rest
         need_x, need_w, need_b = ctx.needs_input_grad[:3]
         dev, cols = x.device, x.shape[-1]
         x2, rows, stride = rows_of(x)
@@ -82,8 +82,8 @@ class _LayerNormFn(torch.autograd.Function):
                 dx = torch.empty(x.shape, dtype=x.dtype, device=dev)
         L = lib()
         if need_w or need_b:
-            dw_direct = flat_grad(wp) if need_w else None
-            db_direct = flat_grad(bp) if need_b else None
+            dw_direct = flat_grad(wp, inner) if need_w else None
+            db_direct = flat_grad(bp, inner) if need_b else None
             new = torch.empty if rows else torch.zeros
             dw, db = dw_direct, db_direct
             if dw is not None:
@@ -104,12 +104,12 @@ class _LayerNormFn(torch.autograd.Function):
                      ptr(w), mean, mean + 4 * rows, ptr(dx), ptr(dw), ptr(db), ptr(ws), ws_bytes,
                      rows, cols, stride, dys, DTYPE_CODES[x.dtype], add, raw_stream(dev.index))
         if dw_direct is not None:
-            last_use_ready(wp, wuse)
+            written(wp)
             dw = None
         elif dw is not None and wp.dtype != torch.float32:
             dw = dw.to(wp.dtype)
         if db_direct is not None:
-            last_use_ready(bp, buse)
+            written(bp)
             db = None
         elif db is not None and bp.dtype != torch.float32:
             db = db.to(bp.dtype)

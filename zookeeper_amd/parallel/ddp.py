@@ -178,7 +178,7 @@ class GradBucketer:
                 self._hooks.append(s.param.register_post_accumulate_grad_hook(hook))
                 # Fused kernels that write gradients in place (bypassing
                 # autograd accumulation) signal completion through this.
-                s.param._zk_grad_ready = lambda h=hook: h(None)
+                s.param._zk_grad_ready = _Ready(self, i, hook)
 
     @property
     def num_buckets(self) -> int:
@@ -413,6 +413,24 @@ class GradBucketer:
         for s in self.flat.slots:
             if hasattr(s.param, "_zk_grad_ready"):
                 del s.param._zk_grad_ready
+
+
+class _Ready:
+    """``param._zk_grad_ready``: called once the parameter's gradient is complete."""
+
+    __slots__ = ("bucketer", "slot", "hook")
+
+    def __init__(self, bucketer: GradBucketer, slot: int, hook):
+        self.bucketer, self.slot, self.hook = bucketer, slot, hook
+
+    def __call__(self) -> None:
+        self.hook(None)
+
+    @property
+    def launched(self) -> bool:
+        """This step's all-reduce of the gradient's bucket has been issued."""
+        b = self.bucketer
+        return b._launched[b.slot_bucket[self.slot]]
 
 
 def order_hash(order: List[int]) -> int:
