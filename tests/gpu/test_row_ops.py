@@ -369,3 +369,33 @@ def test_a_graph_passed_twice_reports_complete_gradients():
         assert torch.equal(flat.grad, want)
         assert sorted(s.name for s, _ in seen) == sorted(s.name for s in flat.slots)
         assert all(torch.equal(g, s.param.grad) for s, g in seen)
+
+
+def test_gradients_that_a_pass_is_not_asked_for():
+    """torch.autograd.grad leaves flat gradients alone and hands out what it names."""
+    model, flat = _shared_model()
+    params = list(model.parameters())
+    x = torch.randn(16, 64, device="cuda", requires_grad=True)
+    flat.zero_grad()
+    z = model(x).square().sum()
+    z.backward(retain_graph=True)
+    torch.cuda.synchronize()
+    want = [p.grad.clone() for p in params]
+    dx = x.grad.clone()
+    flat.zero_grad()
+    assert torch.equal(torch.autograd.grad(z, x, retain_graph=True)[0], dx)
+    z.backward(inputs=[x], retain_graph=True)
+    got = torch.autograd.grad(z, params, retain_graph=True)
+    torch.cuda.synchronize()
+    assert not flat.grad.any()
+    assert all(torch.equal(a, b) for a, b in zip(got, want))
+    # one at a time; the dense bias alone has sums of its own, 16 terms each way
+    tol = 2 * 16 * 2.0 ** -24 * (2 * model(x).detach()).abs().sum(0)
+    for p, a in zip(params, want):
+        tol_p = tol if p is params[-1] else torch.zeros_like(a)
+        assert ((torch.autograd.grad(z, p, retain_graph=True)[0] - a).abs() <= tol_p).all()
+        flat.zero_grad()
+        z.backward(inputs=[p], retain_graph=True)
+        torch.cuda.synchronize()
+        assert ((p.grad - a).abs() <= tol_p).all()
+        assert all(q is p or not q.grad.any() for q in params)

@@ -25,12 +25,11 @@ class _Scale(torch.autograd.Function):
         x, w = ctx.saved_tensors
         p, inner = ctx.rest
         dw = (g * x).sum(0)
-        flat = _rows.flat_grad(p, inner)
+        needed, flat = _rows.flat_grad(ctx, p, inner)
         if flat is not None:
             flat += dw
-            dw = None
             _rows.written(p)
-        return g * w, dw
+        return g * w, dw if needed and flat is None else None
 
 
 class _Layer(torch.nn.Module):
@@ -109,6 +108,26 @@ def test_outside_of_a_pass(layer):
 
     layer.flat.zero_grad()
     _Scale.backward(Ctx, torch.ones(3, 5))
+    assert len(layer.seen) == 1
+
+
+def test_gradients_that_a_pass_is_not_asked_for(layer):
+    """torch.autograd.grad leaves the flat buffer alone and hands out what it names."""
+    def f(m, w):
+        return m(m(X).sin()).sum()
+
+    want = _want(f, layer.w)
+    layer.flat.zero_grad()
+    x = X.clone().requires_grad_(True)
+    z = layer(layer(x).sin()).sum()
+    torch.autograd.grad(z, x, retain_graph=True)
+    z.backward(inputs=[x], retain_graph=True)
+    assert not layer.flat.grad.any() and not layer.seen
+    got, = torch.autograd.grad(z, layer.w, retain_graph=True)
+    torch.testing.assert_close(got, want)
+    assert not layer.flat.grad.any() and not layer.seen
+    z.backward(inputs=[layer.w])
+    torch.testing.assert_close(layer.w.grad, want)
     assert len(layer.seen) == 1
 
 

@@ -157,8 +157,24 @@ def in_backward() -> bool:
     return torch._C._current_graph_task_id() >= 0
 
 
-def flat_grad(p, inner: bool) -> Optional[torch.Tensor]:
-    """:func:`_native.direct_grad` for a parameter that may be used several times in
+def _asked(ctx, p) -> Optional[bool]:
+    """Whether this backward pass accumulates ``p``'s gradient (True), has no use for
+    it (False: ``torch.autograd.grad`` of other tensors, ``backward(inputs=...)``) or
+    hands it to its caller (None: ``torch.autograd.grad`` of ``p``)."""
+    for node, _ in ctx.next_functions:
+        if node is not None and getattr(node, "variable", None) is p:
+            try:
+                return torch._C._will_engine_execute_node(node)
+            except RuntimeError:  # a leaf of torch.autograd.grad
+                return None
+    return True
+
+
+def flat_grad(ctx, p, inner: bool) -> Tuple[bool, Optional[torch.Tensor]]:
+    """``(needed, buffer)``: whether this pass wants ``p``'s gradient, and the flat
+    buffer to add it to (None: return it to autograd).
+
+    :func:`_native.direct_grad` for a parameter that may be used several times in
     one backward pass, on several streams.  Autograd orders the gradients it
     accumulates and knows nothing of these: each write waits for the one before it
     on another stream, and the caller's stream for all of them at the pass's end.
@@ -167,17 +183,21 @@ def flat_grad(p, inner: bool) -> Optional[torch.Tensor]:
     use of the pass (:func:`_accumulated`); ``inner`` (a use recorded in a backward
     pass): not before the bucketer's own end, as only that knows that no further
     inner pass follows.  A write that comes too late all the same raises."""
+    task = torch._C._current_graph_task_id()
+    if task >= 0 and getattr(p, "_zk_direct_grad", False):
+        asked = _asked(ctx, p)
+        if not asked:
+            return asked is None, None
     g = _native.direct_grad(p)
     if g is None:
-        return None
+        return True, None
     ready = getattr(p, "_zk_grad_ready", None)
     if getattr(ready, "launched", False):
         raise RuntimeError(
             "a gradient is written after its all-reduce was launched: the layer is used outside "
             "and inside of a reentrant checkpoint, or twice before the bucketer's finish()")
-    task = torch._C._current_graph_task_id()
     if task < 0:  # not inside a backward pass: one stream, the caller's
-        return g
+        return True, g
     current = _PASSES.get(task)
     if current is None:
         current = _PASSES[task] = _Pass()
@@ -193,7 +213,7 @@ def flat_grad(p, inner: bool) -> Optional[torch.Tensor]:
         hooks = p._post_accumulate_grad_hooks
         if hooks is None or _accumulated not in hooks.values():
             p.register_post_accumulate_grad_hook(_accumulated)
-    return g
+    return True, g
 
 
 def written(p) -> None:

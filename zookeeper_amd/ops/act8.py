@@ -311,8 +311,11 @@ class _Dense8Fn(torch.autograd.Function):
         dx = torch.matmul(dy, weight.to(dy.dtype)) if need_x else None
         dw = db = None
         native = use_kernels(dy, "dense8")
-        dw_direct = flat_grad(wp, ctx.inner) if need_w and native else None
-        db_direct = flat_grad(bp, ctx.inner) if need_b and native else None
+        dw_direct = db_direct = None
+        if need_w and native:
+            need_w, dw_direct = flat_grad(ctx, wp, ctx.inner)
+        if need_b and native:
+            need_b, db_direct = flat_grad(ctx, bp, ctx.inner)
         if need_w and native:
             dw, db = _dense_grads(dy, codes, scales, need_b, dw_direct, db_direct)
         elif need_w:

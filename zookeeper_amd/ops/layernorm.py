@@ -81,9 +81,11 @@ class _LayerNormFn(torch.autograd.Function):
             if need_x:
                 dx = torch.empty(x.shape, dtype=x.dtype, device=dev)
         L = lib()
+        if need_w:
+            need_w, dw_direct = flat_grad(ctx, wp, inner)
+        if need_b:
+            need_b, db_direct = flat_grad(ctx, bp, inner)
         if need_w or need_b:
-            dw_direct = flat_grad(wp, inner) if need_w else None
-            db_direct = flat_grad(bp, inner) if need_b else None
             new = torch.empty if rows else torch.zeros
             dw, db = dw_direct, db_direct
             if dw is not None:
