@@ -306,3 +306,22 @@ def test_large_constant_rows(cols, dt):
     # rstd, the products, the sum's n / 256 + 16 additions and two more roundings; the store
     tol = (cols / 256 + 32) * U32 * mag + _half(dt) * want.abs()
     assert ((dx.double() - want).abs() <= tol).all()
+
+
+@pytest.mark.parametrize("flat", [False, True])
+def test_one_parameter_as_weight_and_bias(flat):
+    from zookeeper_amd.ops import layer_norm
+    from zookeeper_amd.parallel.flat import FlatParams
+
+    torch.manual_seed(10)
+    m = torch.nn.Module()
+    m.p = torch.nn.Parameter(torch.rand(1000, device="cuda"))
+    x, dy = torch.randn(300, 1000, device="cuda"), torch.randn(300, 1000, device="cuda")
+    w = m.p.detach().clone().requires_grad_(True)
+    b = m.p.detach().clone().requires_grad_(True)
+    dw, db = torch.autograd.grad(layer_norm(x, w, b), [w, b], dy)
+    if flat:
+        FlatParams(m).zero_grad()
+    layer_norm(x, m.p, m.p).backward(dy)
+    torch.cuda.synchronize()
+    assert torch.equal(m.p.grad, dw + db)

@@ -85,6 +85,8 @@ class _LayerNormFn(torch.autograd.Function):
             need_w, dw_direct = flat_grad(ctx, wp, inner)
         if need_b:
             need_b, db_direct = flat_grad(ctx, bp, inner)
+        if bp is wp:  # one buffer: two blocks would add to the same elements
+            db_direct = None
         if need_w or need_b:
             new = torch.empty if rows else torch.zeros
             dw, db = dw_direct, db_direct
@@ -106,6 +108,9 @@ class _LayerNormFn(torch.autograd.Function):
                      ptr(w), mean, mean + 4 * rows, ptr(dx), ptr(dw), ptr(db), ptr(ws), ws_bytes,
                      rows, cols, stride, dys, DTYPE_CODES[x.dtype], add, raw_stream(dev.index))
         if dw_direct is not None:
+            if bp is wp:
+                dw_direct += db
+                db = None
             written(wp)
             dw = None
         elif dw is not None and wp.dtype != torch.float32:
