@@ -399,3 +399,35 @@ def test_gradients_that_a_pass_is_not_asked_for():
         torch.cuda.synchronize()
         assert ((p.grad - a).abs() <= tol_p).all()
         assert all(q is p or not q.grad.any() for q in params)
+
+
+class _Fail(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, x):
+        return x.view_as(x)
+
+    @staticmethod
+    def backward(ctx, g):
+        raise ArithmeticError("on purpose")
+
+
+def test_clearing_waits_for_a_failed_pass():
+    """A pass on a side stream fails behind its writes; zero_grad on the caller's stream
+    comes after them all the same."""
+    model, flat = _shared_model()
+    x = torch.randn(256, 64, device="cuda", requires_grad=True)
+    main, side = torch.cuda.current_stream(), torch.cuda.Stream()
+    for _ in range(3):
+        side.wait_stream(main)
+        with torch.cuda.stream(side):
+            z = _Delay.apply(model(_Fail.apply(x)).square()).sum()
+        main.wait_stream(side)
+        with pytest.raises(ArithmeticError):
+            z.backward()
+        flat.zero_grad()
+        got = flat.grad.clone()
+        torch.cuda.synchronize()
+        assert not got.any() and not flat.grad.any()
+    model(x).sum().backward()
+    torch.cuda.synchronize()
+    assert flat.grad.any()

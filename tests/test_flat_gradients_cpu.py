@@ -131,6 +131,26 @@ def test_gradients_that_a_pass_is_not_asked_for(layer):
     assert len(layer.seen) == 1
 
 
+class _Fail(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, x):
+        return x.clone()
+
+    @staticmethod
+    def backward(ctx, g):
+        raise ArithmeticError("on purpose")
+
+
+def test_a_pass_that_fails_leaves_nothing_behind(layer):
+    x = X.clone().requires_grad_(True)
+    for _ in range(2):
+        with pytest.raises(ArithmeticError):
+            layer(_Fail.apply(x)).sum().backward()
+    layer.flat.zero_grad()
+    _check(layer, lambda m, w: m(X).sum())
+    assert not _rows._PASSES and not _rows._FAILED
+
+
 @pytest.fixture
 def bucketer(layer, tmp_path):
     from zookeeper_amd.parallel.ddp import GradBucketer

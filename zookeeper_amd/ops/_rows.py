@@ -107,23 +107,54 @@ def ptr(t):
 
 class _Pass:
     """The flat gradients written in one backward pass: the stream of each
-    parameter's last write, and the parameters written by uses that were recorded
-    inside of another pass.  Called at the pass's end by autograd's engine, which
-    holds the only lasting reference to it."""
+    parameter's last write, the parameters written by uses that were recorded inside
+    of another pass, and the streams of failed passes before it.  Called at the pass's
+    end by autograd's engine, which holds the only lasting reference to it; a pass that
+    fails is not called, only dropped."""
 
-    __slots__ = ("writers", "inner", "__weakref__")
+    __slots__ = ("writers", "inner", "left", "__weakref__")
 
-    def __init__(self):
+    def __init__(self, device: torch.device):
+        self.left = _unjoined(device)
         self.writers: Dict[int, Tuple[torch.device, int]] = {}
         self.inner: Set[int] = set()
 
     def __call__(self):
-        for device, raw in set(self.writers.values()):
-            if raw != _raw(device):
-                torch.cuda.current_stream(device).wait_stream(_stream(device, raw))
+        _wait_for(self.left.union(self.writers.values()))
+        self.left = set()
+        self.writers.clear()
+
+    def __del__(self):
+        _FAILED.update(self.left, self.writers.values())
 
 
 _PASSES: "weakref.WeakValueDictionary[int, _Pass]" = weakref.WeakValueDictionary()
+# Streams of failed passes, whose writes nobody has waited for.
+_FAILED: Set[Tuple[torch.device, int]] = set()
+
+
+def _unjoined(device: torch.device) -> Set[Tuple[torch.device, int]]:
+    """Streams on ``device`` with writes that no ended pass has joined.  (Passes that are
+    still there may be failed ones that the engine has not let go of.)"""
+    left = _FAILED.copy()
+    for current in list(_PASSES.values()):
+        left.update(list(current.writers.values()))
+    if not left or device.type != "cuda" or torch.cuda.is_current_stream_capturing():
+        return set()  # (a capture starts behind a synchronization)
+    return {w for w in left if w[0] == device}
+
+
+def _wait_for(writers) -> None:
+    for device, raw in writers:
+        if raw != _raw(device):
+            torch.cuda.current_stream(device).wait_stream(_stream(device, raw))
+
+
+def join_writers(device: torch.device) -> None:
+    """The current stream waits for the writes that failed passes have left behind:
+    before the buffer is cleared."""
+    _wait_for(_unjoined(device))
+    _FAILED.difference_update([w for w in _FAILED.copy() if w[0] == device])
 
 
 def _raw(device: torch.device) -> int:
@@ -200,13 +231,15 @@ def flat_grad(ctx, p, inner: bool) -> Tuple[bool, Optional[torch.Tensor]]:
         return True, g
     current = _PASSES.get(task)
     if current is None:
-        current = _PASSES[task] = _Pass()
+        current = _PASSES[task] = _Pass(g.device)
         torch.autograd.Variable._execution_engine.queue_callback(current)
     here = (g.device, _raw(g.device))
     last = current.writers.get(id(p), here)
     current.writers[id(p)] = here
     if last != here:
         torch.cuda.current_stream(g.device).wait_stream(_stream(*last))
+    if current.left:
+        _wait_for(current.left)
     if inner:
         current.inner.add(id(p))
     elif ready is not None:

@@ -79,9 +79,10 @@ class FlatParams:
         self.slots = slots
 
     def zero_grad(self) -> None:
-        if self.grad.is_cuda:
-            from zookeeper_amd.ops import _native
+        from zookeeper_amd.ops import _native, _rows
 
+        _rows.join_writers(self.grad.device)
+        if self.grad.is_cuda:
             if _native.available():  # a runtime memset, not a framework fill kernel
                 _native.check(_native.lib().zk_zero(self.grad.data_ptr(),
                                                     self.grad.numel() * 4,
