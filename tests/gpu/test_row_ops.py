@@ -431,3 +431,44 @@ def test_clearing_waits_for_a_failed_pass():
     model(x).sum().backward()
     torch.cuda.synchronize()
     assert flat.grad.any()
+
+
+def test_a_bucket_waits_for_every_stream_that_wrote_it(tmp_path):
+    """Two layers in one bucket, their backwards on two streams: the slow one's gradients
+    are reported first."""
+    import torch.distributed as dist
+
+    from zookeeper_amd import nn as znn
+    from zookeeper_amd.parallel.ddp import GradBucketer
+    from zookeeper_amd.parallel.flat import FlatParams
+
+    torch.manual_seed(11)
+    model = torch.nn.ModuleList([znn.LayerNorm(64), znn.LayerNorm(64)]).cuda()
+    flat = FlatParams(model)
+    x = torch.randn(256, 64, device="cuda")
+    main, side = torch.cuda.current_stream(), torch.cuda.Stream()
+
+    def step():
+        flat.zero_grad()
+        fast = model[0](x).square().sum()
+        side.wait_stream(main)
+        with torch.cuda.stream(side):
+            slow = _Delay.apply(model[1](x).square()).sum()
+        main.wait_stream(side)
+        (fast + slow).backward()
+
+    step()
+    torch.cuda.synchronize()
+    want = flat.grad.clone()
+    dist.init_process_group("gloo", init_method=f"file://{tmp_path}/store", rank=0, world_size=1)
+    bucketer = GradBucketer(flat, world=1, force=True)
+    try:
+        assert bucketer.num_buckets == 1
+        for _ in range(3):
+            step()
+            bucketer.finish()
+            torch.cuda.synchronize()
+            assert torch.equal(flat.grad, want)
+    finally:
+        bucketer.remove()
+        dist.destroy_process_group()

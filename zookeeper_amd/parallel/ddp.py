@@ -20,8 +20,10 @@ Mechanism:
 Stream ordering is explicit and backend-independent (no host
 synchronisation anywhere on the GPU path):
 
-* at bucket-ready an event is recorded on the **compute** stream;
-* a dedicated **comm** HIP stream waits on that event and issues the
+* at bucket-ready an event is recorded on every **compute** stream that
+  reported one of the bucket's gradients (one, unless the backward runs on
+  several);
+* a dedicated **comm** HIP stream waits on those events and issues the
   collective under itself (``torch.distributed`` — backend ``"nccl"`` is
   RCCL — orders its internal stream after the comm stream; gloo's CUDA work
   orders its staging copies the same way);
@@ -57,6 +59,7 @@ from typing import Dict, List, Optional
 import torch
 import torch.distributed as dist
 
+from zookeeper_amd.ops import _rows
 from zookeeper_amd.ops import streams as side_streams
 from zookeeper_amd.parallel.flat import FlatParams
 
@@ -142,6 +145,8 @@ class GradBucketer:
         self._launched = [False] * len(buckets)
         self._hooks = []
         self._seen = [False] * len(flat.slots)
+        # raw streams on which a bucket's gradients were reported ready
+        self._reporters = [set() for _ in buckets]
         self._suspended = False
         self.enabled = world > 1 or bool(force)
         if self.enabled and not (dist.is_available() and dist.is_initialized()):
@@ -211,6 +216,7 @@ class GradBucketer:
         finally:
             self._suspended = old
             self._seen = [False] * len(self.flat.slots)
+            self._reporters = [set() for _ in self.buckets]
             self._pending = [len(b) for b in self.buckets]
             self._clear_claims()
 
@@ -237,6 +243,8 @@ class GradBucketer:
                 return
             self._seen[slot_index] = True
             b = self.slot_bucket[slot_index]
+            if self.comm_stream is not None:
+                self._reporters[b].add(_rows._raw(self.flat.grad.device))
             self._pending[b] -= 1
             if self._pending[b] == 0:
                 self._launch(b)
@@ -262,6 +270,11 @@ class GradBucketer:
         ready = torch.cuda.Event()
         ready.record(torch.cuda.current_stream(view.device))
         self.comm_stream.wait_event(ready)
+        # the streams of the gradients reported before the last one
+        here = _rows._raw(view.device)
+        for raw in self._reporters[b]:
+            if raw != here:
+                self.comm_stream.wait_stream(_rows._stream(view.device, raw))
         # this bucket's weight gradients still running on the side stream
         # (ops/streams.py); the other buckets' are not waited for
         for ev in side_streams.unwaited_events_for(self._bucket_pids[b]):
@@ -369,6 +382,7 @@ class GradBucketer:
         self._pending = [len(b) for b in self.buckets]
         self._launched = [False] * len(self.buckets)
         self._seen = [False] * len(self.flat.slots)
+        self._reporters = [set() for _ in self.buckets]
         self._clear_claims()
 
     def compare_order(self, order: List[int]) -> None:
