@@ -189,7 +189,7 @@ class _Gelu8Fn(torch.autograd.Function):
     def backward(ctx, dy):
         if torch.is_grad_enabled():
             refuse_twice("gelu8")
-        kept, = ctx.saved_tensors
+        kept = ctx.saved_tensors[0].contiguous()  # hooks may have changed the layout
         n, rows, dev = dy.shape[-1], ctx.rows, dy.device
         if dy.is_contiguous():
             dx, dy2, stride = torch.empty_like(dy), dy, n
@@ -316,10 +316,12 @@ class _Dense8Fn(torch.autograd.Function):
             need_w, dw_direct = flat_grad(ctx, wp, ctx.inner)
         if need_b and native:
             need_b, db_direct = flat_grad(ctx, bp, ctx.inner)
-        if need_w and native:
-            dw, db = _dense_grads(dy, codes, scales, need_b, dw_direct, db_direct)
+        if need_w and native:  # contiguous: hooks may have changed the layout
+            dw, db = _dense_grads(dy, codes.contiguous(), scales.contiguous(), need_b, dw_direct,
+                                  db_direct)
         elif need_w:
-            dw, db = dense8_grads(dy, Packed8(codes, scales, dy.dtype), need_b)
+            dw, db = dense8_grads(dy, Packed8(codes.contiguous(), scales.contiguous(), dy.dtype),
+                                  need_b)
         elif need_b:  # a frozen weight with a trainable bias
             db = dy.reshape(-1, dy.shape[-1]).float().sum(0)
             if db_direct is not None:

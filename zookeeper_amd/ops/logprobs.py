@@ -84,7 +84,9 @@ class _TokenLogProbsFn(torch.autograd.Function):
             return None, None, None, None
         logits, tokens = ctx.saved_tensors
         stats, ignore = ctx.rest
-        x, rows, stride = rows_of(logits)  # anew: hooks on saved tensors may change the layout
+        # anew: hooks on saved tensors may change the layout
+        x, rows, stride = rows_of(logits)
+        tokens = tokens.contiguous()
         if logits.is_contiguous():
             dx = torch.empty_like(logits)
         else:
