@@ -288,11 +288,23 @@ def dense8_grads(dy: torch.Tensor, kept: Packed8,
     return d.t() @ x, d.sum(0) if bias else None
 
 
+def _product(f, x, *operands):
+    """``f(x, *operands)`` with the rows of ``x`` as one matrix.  torch makes a batched
+    product of rows that do not merge, with a transposed view as its right operand, a
+    form that has faulted in bfloat16."""
+    if x.dim() <= 2:
+        return f(x, *operands)
+    return f(x.reshape(-1, x.shape[-1]), *operands).unflatten(0, x.shape[:-1])
+
+
+def _linear(x, weight, bias):
+    return _product(F.linear, x, weight.to(x.dtype), bias.to(x.dtype) if bias is not None else None)
+
+
 class _Dense8Fn(torch.autograd.Function):
     @staticmethod
     def forward(ctx, x, weight, bias):
-        w = weight.to(x.dtype)
-        y = F.linear(x, w, bias.to(x.dtype) if bias is not None else None)
+        y = _linear(x, weight, bias)
         codes = scales = None
         if ctx.needs_input_grad[1]:
             codes, scales = _pack(x) if use_kernels(x, "dense8") else _pack_plain(x)
@@ -308,7 +320,7 @@ class _Dense8Fn(torch.autograd.Function):
         codes, scales, weight = ctx.saved_tensors
         need_x, need_w, need_b = ctx.needs_input_grad
         wp, bp = ctx.weight_param, ctx.bias_param
-        dx = torch.matmul(dy, weight.to(dy.dtype)) if need_x else None
+        dx = _product(torch.matmul, dy, weight.to(dy.dtype)) if need_x else None
         dw = db = None
         native = use_kernels(dy, "dense8")
         dw_direct = db_direct = None
@@ -360,4 +372,4 @@ def dense8(x: torch.Tensor, weight: torch.Tensor,
     if torch.is_grad_enabled() and (x.requires_grad or weight.requires_grad
                                     or (bias is not None and bias.requires_grad)):
         return _Dense8Fn.apply(x, weight, bias)
-    return F.linear(x, weight.to(x.dtype), bias.to(x.dtype) if bias is not None else None)
+    return _linear(x, weight, bias)
