@@ -148,7 +148,8 @@ def test_dense_products_are_no_batched_ones(bias, recorded):
               base[:0]):
         v = x.detach().requires_grad_(recorded)
         wr = w.detach().requires_grad_(recorded)
-        dy = torch.randn(7, *reversed(x.shape[:-1])).permute(*reversed(range(x.dim())))
+        dy = torch.randn(*reversed(x.shape[:-1]), 7)
+        dy = dy.permute(*reversed(range(x.dim() - 1)), -1)
         with Calls():
             y = dense8(v, wr, b)
             grads = torch.autograd.grad(y, [v, wr], dy) if recorded else ()
