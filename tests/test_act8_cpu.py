@@ -126,9 +126,10 @@ def test_steps_under_the_smallest_packed_one():
     assert torch.equal(dw.double(), want * 2.0 ** 100)
 
 
+@pytest.mark.parametrize("dt", [torch.float32, torch.bfloat16])
 @pytest.mark.parametrize("recorded", [False, True])
 @pytest.mark.parametrize("bias", [False, True])
-def test_dense_products_are_no_batched_ones(bias, recorded):
+def test_dense_products_are_no_batched_ones(bias, recorded, dt):
     """Rows that do not merge (permuted, broadcast) are copied to one matrix: torch's
     batched product would take the weight as a transposed view."""
     from torch.utils._python_dispatch import TorchDispatchMode
@@ -143,18 +144,20 @@ def test_dense_products_are_no_batched_ones(bias, recorded):
     torch.manual_seed(3)
     w = torch.randn(40, 7).t()  # itself a transposed view
     b = torch.randn(7) if bias else None
-    base = torch.randn(6, 5, 40)
+    base = torch.randn(6, 5, 40).to(dt)
     for x in (base, base.transpose(0, 1), base[:1].expand(4, 5, 40), base[0], base[0, 0],
               base[:0]):
         v = x.detach().requires_grad_(recorded)
         wr = w.detach().requires_grad_(recorded)
         dy = torch.randn(*reversed(x.shape[:-1]), 7)
-        dy = dy.permute(*reversed(range(x.dim() - 1)), -1)
+        dy = dy.permute(*reversed(range(x.dim() - 1)), -1).to(dt)
         with Calls():
             y = dense8(v, wr, b)
             grads = torch.autograd.grad(y, [v, wr], dy) if recorded else ()
-        torch.testing.assert_close(y, torch.nn.functional.linear(x, w, b))
-        if recorded:
-            assert grads[0].shape == x.shape
-            torch.testing.assert_close(grads[0], dy @ w)
+        assert y.shape == (*x.shape[:-1], 7) and all(g.shape == u.shape
+                                                     for g, u in zip(grads, (x, w)))
+        if dt == torch.float32:
+            torch.testing.assert_close(y, torch.nn.functional.linear(x, w, b))
+            if recorded:
+                torch.testing.assert_close(grads[0], dy @ w)
     assert any("mm" in f for f in Calls.seen) and not any("bmm" in f for f in Calls.seen)
