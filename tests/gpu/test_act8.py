@@ -529,3 +529,45 @@ def test_small_steps_in_the_weight_gradient(dt, variant):
     zero = torch.zeros_like(kept.codes)
     dw, _ = _dense_grads(dy, zero, torch.zeros_like(kept.scales), True, variant=variant)
     assert torch.equal(dw, torch.zeros_like(dw))
+
+
+@pytest.mark.parametrize("flat", [False, True])
+@pytest.mark.parametrize("rows,outs,dt", [(1, 5, torch.float32), (5000, 33, torch.float16),
+                                          (100000, 7, torch.bfloat16)])
+def test_bias_of_a_frozen_weight_replays_in_a_graph(rows, outs, dt, flat):
+    from zookeeper_amd.ops import dense8
+    from zookeeper_amd.parallel.flat import FlatParams
+
+    torch.manual_seed(rows)
+    m = torch.nn.Module()
+    m.b = torch.nn.Parameter(torch.randn(outs, device="cuda"))
+    w = torch.randn(outs, 20, device="cuda")
+    if flat:
+        f = FlatParams(m)
+    x = torch.zeros(rows, 20, device="cuda", dtype=dt)
+    dy = torch.zeros(rows, outs, device="cuda", dtype=dt)
+
+    def step():
+        if flat:
+            m.b.grad.zero_()
+            dense8(x, w, m.b).backward(dy)
+            return m.b.grad
+        return torch.autograd.grad(dense8(x, w, m.b), m.b, dy)[0]
+
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        step()
+    torch.cuda.current_stream().wait_stream(side)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        out = step()
+    for i in range(4):
+        dy.copy_(torch.randn(rows, outs, device="cuda").to(dt))
+        graph.replay()
+        torch.cuda.synchronize()
+        got = out.clone()
+        want, mag = dy.double().sum(0), dy.double().abs().sum(0)
+        assert ((got.double() - want).abs() <= (rows + 16) * 2.0 ** -23 * mag).all(), i
+        assert torch.equal(step(), got), i
+        torch.cuda.synchronize()

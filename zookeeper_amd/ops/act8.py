@@ -334,10 +334,11 @@ class _Dense8Fn(torch.autograd.Function):
         elif need_w:
             dw, db = dense8_grads(dy, Packed8(codes.contiguous(), scales.contiguous(), dy.dtype),
                                   need_b)
-        elif need_b:  # a frozen weight with a trainable bias
+        elif need_b and native:  # a frozen weight with a trainable bias: of a column of zeros
+            none = torch.zeros((dy.numel() // dy.shape[-1], 1), dtype=torch.int8, device=dy.device)
+            _, db = _dense_grads(dy, none, none.view(torch.uint8), True, None, db_direct)
+        elif need_b:
             db = dy.reshape(-1, dy.shape[-1]).float().sum(0)
-            if db_direct is not None:
-                db_direct += db
         if dw_direct is not None:
             written(wp)
             dw = None
