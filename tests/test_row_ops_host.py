@@ -1,6 +1,7 @@
 """The row operators on hosts without a GPU."""
 
 import os
+import re
 import subprocess
 import sys
 
@@ -29,3 +30,13 @@ def test_a_torch_without_gpu_bindings(tmp_path):
     run = subprocess.run([sys.executable, "-c", PROGRAM], capture_output=True, text=True,
                          cwd=str(tmp_path), env=dict(os.environ, PYTHONPATH=ROOT), timeout=300)
     assert run.returncode == 0 and run.stdout.strip().endswith("done"), run.stderr[-2000:]
+
+
+def test_no_shared_state_without_atomics():
+    """The C entries are called from several host threads (the calls release the GIL): what
+    they keep between calls is atomic or constant."""
+    for name in ("act8.hip", "layer_norm.hip", "logprobs.hip", "rows.h"):
+        with open(os.path.join(ROOT, "zookeeper_amd", "csrc", "kernels", name)) as f:
+            for line in f:
+                m = re.match(r"\s*static\s+(?!const|constexpr|__device__|std::atomic)(.*)", line)
+                assert not m or re.match(r"[\w:<> *&]+\(", m.group(1)), (name, line)

@@ -21,6 +21,8 @@
 // 8192 bf16: pack 73 us, unpack 75 us (5.5 TB/s), GELU with its kept input 159 us,
 // GELU backward 155 us (4.3 TB/s: their 31 instructions a value, two of them
 // transcendental, take nearly as long; fp32 runs at 5.9 TB/s).
+#include <atomic>
+
 #include "mfma_common.h"
 #include "rows.h"
 
@@ -958,17 +960,18 @@ bool dense8_ok(long long M, int N, int K, long long dys) {
 }
 
 int dense8_wide_launch(const D8WideArgs& a, hipStream_t st) {
-  static bool ready[64];  // by device: over 64 KB of LDS are allowed per kernel and device
+  // by device: over 64 KB of LDS are allowed per kernel and device (twice does no harm)
+  static std::atomic<bool> ready[64];
   int dev = 0;
   hipError_t e = hipGetDevice(&dev);
   if (e != hipSuccess) return (int)e;
-  if (dev < 0 || dev >= 64 || !ready[dev]) {
+  if (dev < 0 || dev >= 64 || !ready[dev].load(std::memory_order_acquire)) {
     for (const void* f :
          {(const void*)dense8_wide_kernel<false>, (const void*)dense8_wide_kernel<true>}) {
       e = hipFuncSetAttribute(f, hipFuncAttributeMaxDynamicSharedMemorySize, kWLds);
       if (e != hipSuccess) return (int)e;
     }
-    if (dev >= 0 && dev < 64) ready[dev] = true;
+    if (dev >= 0 && dev < 64) ready[dev].store(true, std::memory_order_release);
   }
   const dim3 g((unsigned)(a.ntiles * a.ktiles * a.splits));
   if (a.K & 7)
