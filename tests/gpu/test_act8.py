@@ -571,3 +571,15 @@ def test_bias_of_a_frozen_weight_replays_in_a_graph(rows, outs, dt, flat):
         assert ((got.double() - want).abs() <= (rows + 16) * 2.0 ** -23 * mag).all(), i
         assert torch.equal(step(), got), i
         torch.cuda.synchronize()
+
+
+@pytest.mark.parametrize("shape", [(0, 40), (3, 0), (0, 0), (0,)])
+def test_a_form_of_nothing(shape):
+    """What the constructor takes unpacks, as on the host."""
+    from zookeeper_amd.ops import Packed8, unpack8
+
+    for device in ("cuda", "cpu"):
+        codes = torch.zeros(shape, dtype=torch.int8, device=device)
+        scales = torch.zeros((*shape[:-1], -(-shape[-1] // 32)), dtype=torch.uint8, device=device)
+        out = unpack8(Packed8(codes, scales, torch.bfloat16))
+        assert out.shape == shape and out.dtype == torch.bfloat16

@@ -150,6 +150,8 @@ def unpack8(kept: Packed8, dtype: Optional[torch.dtype] = None) -> torch.Tensor:
     if not use_kernels(out, "unpack8"):
         return _unpack_plain(kept.codes, kept.scales, dtype)
     refuse_tracing("unpack8")
+    if out.numel() == 0:
+        return out
     n = kept.shape[-1]
     with guard(out):
         call(lib().zk_unpack8, "zk_unpack8", kept.codes.data_ptr(), kept.scales.data_ptr(),
