@@ -60,3 +60,12 @@ def test_refusals():
         token_logprobs(torch.randn(3, 100), t, top=65)
     with pytest.raises(ValueError, match="floating"):
         token_logprobs(x.int(), t)
+
+
+def test_ignored_index_of_more_than_64_bits():
+    """2^64 - 100 would be -100 in the kernels."""
+    x, t = torch.randn(3, 5), torch.tensor([0, -100, 4])
+    for index in (2 ** 64 - 100, 2 ** 63, -2 ** 63 - 1):
+        with pytest.raises(ValueError, match="64-bit"):
+            token_logprobs(x, t, ignore_index=index)
+    assert token_logprobs(x, t, ignore_index=-2 ** 63).logp[1].isnan()

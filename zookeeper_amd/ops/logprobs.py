@@ -148,6 +148,8 @@ def token_logprobs(logits: torch.Tensor, tokens: torch.Tensor, top: int = 0,
     if not 0 <= top <= min(MAX_TOP, logits.shape[-1]):
         raise ValueError(f"token_logprobs: top must be in [0, {min(MAX_TOP, logits.shape[-1])}], "
                          f"got {top}")
+    if not -2 ** 63 <= ignore_index < 2 ** 63:
+        raise ValueError(f"token_logprobs: ignore_index {ignore_index} is no 64-bit number")
     if not use_kernels(logits, "token_logprobs"):
         return _plain(logits, tokens, top, ignore_index)
     if logits.shape[-1] >= 0x7FFF0000:
