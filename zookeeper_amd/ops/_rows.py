@@ -21,6 +21,9 @@ _FLOATS = (torch.float32, torch.bfloat16, torch.float16, torch.float64)
 # Raw hipStream_t of torch's current stream on a device index (a torch without GPU
 # support lacks the name, and has no GPU tensors to need it).
 raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None)
+# The backward pass that this thread runs, -1 for none.
+_task = torch._C._current_graph_task_id
+_is_tracing = torch._C._is_tracing
 
 _HERE = contextlib.nullcontext()
 
@@ -51,11 +54,11 @@ def tracked() -> bool:
     """True while torch follows calls by other means than ``requires_grad``: tracing
     records an autograd function as one call, and forward-mode differentiation
     is refused by it.  A bare launch would be invisible to both."""
-    return forward_ad._current_level >= 0 or torch._C._is_tracing()
+    return forward_ad._current_level >= 0 or _is_tracing()
 
 
 def refuse_tracing(what: str) -> None:
-    if torch._C._is_tracing():
+    if _is_tracing():
         raise RuntimeError(f"{what}: cannot be traced (it is no autograd function)")
 
 
@@ -171,7 +174,7 @@ def _accumulated(p) -> None:
     """Autograd's hook behind the last use of ``p`` in a backward pass, whichever
     uses that pass has: every write into its flat gradient is enqueued, each behind
     the one before, so the bucketer may have it from the last one's stream on."""
-    current = _PASSES.get(torch._C._current_graph_task_id())
+    current = _PASSES.get(_task())
     last = current.writers.get(id(p)) if current is not None else None
     if last is None or id(p) in current.inner:
         return
@@ -185,7 +188,7 @@ def _accumulated(p) -> None:
 def in_backward() -> bool:
     """True inside a backward pass.  A use recorded there belongs to a pass of its own
     inside that one (reentrant checkpointing), and others may follow."""
-    return torch._C._current_graph_task_id() >= 0
+    return _task() >= 0
 
 
 def _asked(ctx, p) -> Optional[bool]:
@@ -214,7 +217,7 @@ def flat_grad(ctx, p, inner: bool) -> Tuple[bool, Optional[torch.Tensor]]:
     use of the pass (:func:`_accumulated`); ``inner`` (a use recorded in a backward
     pass): not before the bucketer's own end, as only that knows that no further
     inner pass follows.  A write that comes too late all the same raises."""
-    task = torch._C._current_graph_task_id()
+    task = _task()
     if task >= 0 and getattr(p, "_zk_direct_grad", False):
         asked = _asked(ctx, p)
         if not asked:
@@ -251,7 +254,7 @@ def flat_grad(ctx, p, inner: bool) -> Tuple[bool, Optional[torch.Tensor]]:
 
 def written(p) -> None:
     """After a write into ``p``'s flat gradient outside of any backward pass."""
-    if torch._C._current_graph_task_id() < 0:
+    if _task() < 0:
         _native.grad_ready(p)
 
 
