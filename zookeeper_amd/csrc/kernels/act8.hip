@@ -18,9 +18,10 @@
 //
 // All elementwise kernels are bound by memory.  A lane owns 8 values, the four
 // lanes of a quad a block: the block's maximum takes two DPP moves.  Measured, 16384 x
-// 8192 bf16: pack 73 us, unpack 75 us (5.5 TB/s), GELU with its kept input 159 us,
-// GELU backward 155 us (4.3 TB/s: their 31 instructions a value, two of them
-// transcendental, take nearly as long; fp32 runs at 5.9 TB/s).
+// 8192 bf16, each back to back with itself: pack 76 us, unpack 72 us (5.4 TB/s), GELU
+// with its kept input 128 us, GELU backward 165 us (4.1 TB/s: its 31 instructions a value,
+// two of them transcendental, take nearly as long; fp32 208 and 207 us, 5.8 TB/s).  The
+// two passes of GELU in turn take 275 us.
 #include <atomic>
 
 #include "mfma_common.h"
@@ -234,9 +235,9 @@ int act8_launch(const void* in, void* out, void* codes, void* scales, long long 
 // Few tiles: the rows are split, every split writes its partial tile and a
 // second launch adds them in order (no atomics).
 //
-// This kernel serves the smaller sizes (1024 x 1024 x 1024 bf16 27 us, 256 x 1024 x
-// 1024 16 us: the start and end of a block and the partial sums); at large ones it is
-// bound by its own staging (16384 x 4096 x 4096 1437 us, 0.38 PFLOP/s).
+// This kernel serves the smaller sizes (1024 x 1024 x 1024 bf16 26 us, 256 x 1024 x
+// 1024 17 us: the start and end of a block and the partial sums); at large ones it is
+// bound by its own staging (16384 x 4096 x 4096 1448 us, 0.38 PFLOP/s).
 // ===========================================================================
 typedef float f32x4 __attribute__((ext_vector_type(4)));
 
@@ -479,8 +480,9 @@ __global__ __launch_bounds__(kNT, 2) void dense8_wgrad_kernel(D8Args a) {
 // [term][Mp][N8], and the product runs over the terms one after the other (virtual
 // row r: kept row r mod Mp).
 //
-// Measured: 16384 x 4096 x 4096 bf16 523 - 548 us over several machines (1.0 PFLOP/s; the
-// library's product of the same shape with a bf16 input 559), fp16 1093, fp32 1602.
+// Measured: 16384 x 4096 x 4096 bf16 500 - 548 us over several machines (1.0 - 1.1
+// PFLOP/s; the library's product of the same shape with a bf16 input 460, 555 on its
+// first calls), fp16 1033 - 1093, fp32 1592 - 1602.
 // ---------------------------------------------------------------------------
 constexpr int kW = 256;                 // tile edge
 constexpr int kWNT = 512;               // threads
@@ -906,9 +908,9 @@ struct D8Plan {
 D8Plan dense8_plan(long long M, int N, int K, int dt, long long dys, bool aligned, int variant) {
   D8Plan p{};
   // us per call, 128 / 256 kernel (rows x outputs x inputs, bf16): 1024 x 1024 x 1024
-  // 27 / 42, 4096 x 512 x 512 31 / 33, 16384 x 1024 x 128 33 / 37, 32768 x 256 x 512
-  // 44 / 44, 512 x 2048 x 2048 35 / 29, 4096 x 768 x 768 58 / 38, 16384 x 1024 x 1024
-  // 99 / 64, 16384 x 4096 x 4096 1437 / 535.
+  // 26 / 42, 4096 x 512 x 512 30 / 32, 16384 x 1024 x 128 30 / 36, 32768 x 256 x 512
+  // 39 / 43, 512 x 2048 x 2048 31 / 30, 4096 x 768 x 768 45 / 37, 16384 x 1024 x 1024
+  // 99 / 64, 16384 x 4096 x 4096 1448 / 498.
   p.wide = variant == 1 || (variant < 0 && M >= 64 && N >= 192 && K >= 192 &&
                             (long long)N * K >= (1 << 18) &&
                             (double)M * N * K >= 2147483648.0);

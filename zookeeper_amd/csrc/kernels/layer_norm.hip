@@ -12,10 +12,14 @@
 // registers, no E[x^2] - mean^2).  Both passes are bound by memory: forward
 // x + y, backward x + dy + dx, everything else stays in registers.  A row
 // belongs to G lanes that hold it whole: NV vectors of 8 elements per lane.
-// Rows over 16384 elements take the looping kernels, which read a row again
-// (it is then in L2).  Measured, 32768 x 2048 bf16: forward 50 us (5.3 TB/s),
-// backward 84 us (4.8 TB/s, of which 5 us for the join of dw / db); 4096 x 16384
-// 51 and 88 us; 1000000 x 16 fp32 22 and 36 us; a device copy runs at 5.2 TB/s.
+// Measured, 32768 x 2048 bf16: forward 52 us (5.1 TB/s), backward 84 us (4.8 TB/s, of
+// which 5 us for the join of dw / db); 4096 x 16384 51 and 92 us; 1000000 x 16 fp32 23
+// and 37 us; a device copy runs at 5.2 TB/s.
+//
+// Rows over 16384 elements take the looping kernels: three sweeps of x forward, three
+// of x and dy backward, which the L2s hold in part only.  4096 x 32768 bf16 180 and 372 us
+// (3.0 and 2.2 TB/s of x + y and x + dy + dx), fp32 394 and 661 us; 512 x 65536 bf16 55
+// and 107 us.
 //
 // dw / db: blocks walk rows with a fixed stride and keep their columns' sums in
 // registers; the lane groups of a block are joined through LDS, each block
