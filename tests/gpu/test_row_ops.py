@@ -498,3 +498,44 @@ def test_saved_tensors_may_come_back_with_gaps(device):
         got = run()
     for p, q in zip(got, want):  # the host's reductions may round otherwise by layout
         assert torch.equal(p, q) if device == "cuda" else torch.allclose(p, q, rtol=1e-4, atol=1e-5)
+
+
+@pytest.mark.parametrize("segments", [None, False, True])
+def test_steps_under_the_bucketer(tmp_path, segments):
+    """Plain and checkpointed (not reentrant, reentrant) layers, one of them shared: the
+    reduced gradients of several steps are those without data parallelism."""
+    import torch.distributed as dist
+    from torch.utils.checkpoint import checkpoint
+
+    from zookeeper_amd import nn as znn
+    from zookeeper_amd.parallel.ddp import GradBucketer
+    from zookeeper_amd.parallel.flat import FlatParams
+
+    torch.manual_seed(13)
+    layer = torch.nn.Sequential(znn.LayerNorm(64), znn.GELU(kept="int8"),
+                                znn.QuantDense(64, 64, use_bias=True, kept="int8"))
+    head = znn.QuantDense(64, 10, use_bias=True, kept="int8")
+    flat = FlatParams(torch.nn.ModuleList([layer, head]).cuda())
+    batches = [torch.randn(200, 64, device="cuda") for _ in range(3)]
+
+    def step(x, bucketer=None):
+        flat.zero_grad()
+        h = x.clone().requires_grad_(True)
+        for _ in range(3):
+            h = h + (layer(h) if segments is None else checkpoint(layer, h, use_reentrant=segments))
+        head(h).square().sum().backward()
+        if bucketer is not None:
+            bucketer.finish()
+        torch.cuda.synchronize()
+        return flat.grad.clone()
+
+    want = [step(x) for x in batches]
+    dist.init_process_group("gloo", init_method=f"file://{tmp_path}/store", rank=0, world_size=1)
+    bucketer = GradBucketer(flat, world=1, force=True, bucket_mb=0.001, first_bucket_mb=0.001)
+    try:
+        assert bucketer.num_buckets > 1
+        for x, w in zip(batches, want):
+            assert torch.equal(step(x, bucketer), w)
+    finally:
+        bucketer.remove()
+        dist.destroy_process_group()
