@@ -151,6 +151,27 @@ def test_a_pass_that_fails_leaves_nothing_behind(layer):
     assert not _rows._PASSES and not _rows._FAILED
 
 
+def test_captured_passes_are_not_waited_for(monkeypatch):
+    """Another thread's eager pass beside one that is captured, and the reverse."""
+    device = torch.device("cuda", 0)
+    state = {"capturing": False}
+    monkeypatch.setattr(torch.cuda, "is_current_stream_capturing", lambda: state["capturing"])
+    eager = _rows._PASSES[-10] = _rows._Pass(device)
+    eager.writers[1] = (device, 17)
+    state["capturing"] = True
+    captured = _rows._PASSES[-11] = _rows._Pass(device)
+    captured.writers[1] = (device, 18)
+    assert not captured.left and not _rows._unjoined(device)
+    state["capturing"] = False
+    assert _rows._unjoined(device) == {(device, 17)}
+    assert not _rows._unjoined(torch.device("cuda", 1))
+    del captured
+    assert not _rows._FAILED
+    del eager  # failed
+    assert _rows._FAILED == {(device, 17)} and not _rows._PASSES
+    _rows._FAILED.clear()
+
+
 @pytest.fixture
 def bucketer(layer, tmp_path):
     from zookeeper_amd.parallel.ddp import GradBucketer

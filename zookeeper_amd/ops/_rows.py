@@ -115,10 +115,13 @@ class _Pass:
     end by autograd's engine, which holds the only lasting reference to it; a pass that
     fails is not called, only dropped."""
 
-    __slots__ = ("writers", "inner", "left", "__weakref__")
+    __slots__ = ("writers", "inner", "left", "captured", "__weakref__")
 
     def __init__(self, device: torch.device):
-        self.left = _unjoined(device)
+        # a captured pass runs at its replays: nothing to wait for, and to wait for its
+        # stream would draw the waiting one into the capture
+        self.captured = _capturing(device)
+        self.left = set() if self.captured else _unjoined(device)
         self.writers: Dict[int, Tuple[torch.device, int]] = {}
         self.inner: Set[int] = set()
 
@@ -128,7 +131,8 @@ class _Pass:
         self.writers.clear()
 
     def __del__(self):
-        _FAILED.update(self.left, self.writers.values())
+        if not self.captured:
+            _FAILED.update(self.left, self.writers.values())
 
 
 _PASSES: "weakref.WeakValueDictionary[int, _Pass]" = weakref.WeakValueDictionary()
@@ -141,10 +145,15 @@ def _unjoined(device: torch.device) -> Set[Tuple[torch.device, int]]:
     still there may be failed ones that the engine has not let go of.)"""
     left = _FAILED.copy()
     for current in list(_PASSES.values()):
-        left.update(list(current.writers.values()))
-    if not left or device.type != "cuda" or torch.cuda.is_current_stream_capturing():
-        return set()  # (a capture starts behind a synchronization)
-    return {w for w in left if w[0] == device}
+        if not current.captured:
+            left.update(list(current.writers.values()))
+    left = {w for w in left if w[0] == device}
+    # (a capture starts behind a synchronization)
+    return set() if left and _capturing(device) else left
+
+
+def _capturing(device: torch.device) -> bool:
+    return device.type == "cuda" and torch.cuda.is_current_stream_capturing()
 
 
 def _wait_for(writers) -> None:
